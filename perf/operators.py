@@ -1,0 +1,381 @@
+"""Cases for measuring the operators of an attention decoder's step: appending to a paged key-value cache with the
+position rotation (`PagedCache.append`), attention of one new token over that cache (`PagedCache.attend`) and matrix-vector
+products with 4-bit weights (`W4Matrix.matvec`).  `run` computes a case with the framework's kernels where `own` is set and
+in plain torch operations where it is not; `exact` computes it from the definition in 64 bits.
+
+Sizes come from the Tacotron 2 checkpoints this framework serves where there is a counterpart (1024-wide states, 1558
+inputs and 4096 gate rows of the decoder LSTM, 80 mel channels, sixteen lines in flight, up to 3000 frames a line) and are
+generic otherwise."""
+import math
+import random
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+_BYTES = {"f32": 4, "f16": 2, "bf16": 2, "e4m3": 1}
+_DEV = "cuda:0"
+
+
+def listed():
+  return [
+    # the next frame of a lone line: sixteen heads of a 1024-wide state
+    {"name": "append_line_f32", "op": "append", "dtype": "f32", "cache": "f32", "seqs": 1, "new": 1, "past": 700, "hq": 16,
+     "hkv": 16, "d": 64, "page": 16, "rot": 64, "interleaved": False},
+    # one frame of a batch of 64 lines, grouped heads
+    {"name": "append_batch_bf16", "op": "append", "dtype": "bf16", "cache": "bf16", "seqs": 64, "new": 1, "past": 3000,
+     "hq": 32, "hkv": 8, "d": 128, "page": 64, "rot": 128, "interleaved": False},
+    # ragged prompts at far positions into an 8-bit cache, neighbouring pairs rotated
+    {"name": "append_prompts_e4m3", "op": "append", "dtype": "bf16", "cache": "e4m3", "seqs": 7, "new": 1601, "past": 120001,
+     "hq": 32, "hkv": 8, "d": 128, "page": 32, "rot": 64, "interleaved": True},
+    # a lone line again: one query over 777 frames
+    {"name": "attend_line_f32", "op": "attend", "dtype": "f32", "cache": "f32", "seqs": 1, "len": 777, "hq": 16, "hkv": 16,
+     "d": 64, "page": 16, "window": 0},
+    # sixteen lines in flight, every head with keys of its own
+    {"name": "attend_lines_f16", "op": "attend", "dtype": "f16", "cache": "f16", "seqs": 16, "len": 3000, "hq": 16, "hkv": 16,
+     "d": 64, "page": 16, "window": 0},
+    # a batch of 64 ragged sequences, four queries to a key head
+    {"name": "attend_batch_bf16", "op": "attend", "dtype": "bf16", "cache": "bf16", "seqs": 64, "len": 8191, "hq": 32,
+     "hkv": 8, "d": 128, "page": 64, "window": 0},
+    # one long sequence: all of the card's work comes from splitting its length
+    {"name": "attend_long_bf16", "op": "attend", "dtype": "bf16", "cache": "bf16", "seqs": 1, "len": 131075, "hq": 32,
+     "hkv": 8, "d": 128, "page": 256, "window": 0},
+    # an 8-bit cache, a window that hides the far past of the long ones
+    {"name": "attend_window_e4m3", "op": "attend", "dtype": "bf16", "cache": "e4m3", "seqs": 33, "len": 20000, "hq": 64,
+     "hkv": 8, "d": 128, "page": 32, "window": 12000},
+    # the mel projection of one frame
+    {"name": "w4_projection_f32", "op": "w4", "dtype": "f32", "scales": "f32", "m": 1, "n": 80, "k": 1558, "group": 32,
+     "zeros": False, "bias": True},
+    # the gate rows of an LSTM cell for sixteen lines in flight
+    {"name": "w4_gates_f32", "op": "w4", "dtype": "f32", "scales": "f32", "m": 16, "n": 4096, "k": 1558, "group": 64,
+     "zeros": False, "bias": True},
+    # a square projection of one token
+    {"name": "w4_square_f16", "op": "w4", "dtype": "f16", "scales": "f16", "m": 1, "n": 4096, "k": 4096, "group": 128,
+     "zeros": False, "bias": False},
+    # the wide layer of a large model, one token
+    {"name": "w4_wide_bf16", "op": "w4", "dtype": "bf16", "scales": "bf16", "m": 1, "n": 28672, "k": 8192, "group": 128,
+     "zeros": True, "bias": False},
+  ]
+
+
+def _log(rng, lo, hi):
+  return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+  op = rng.choice(["append", "attend", "attend", "w4", "w4"])
+  if op == "w4":
+    dtype = rng.choice(["f32", "f16", "bf16"])
+    while True:
+      c = {"op": op, "dtype": dtype, "scales": rng.choice([dtype, "f32"]), "m": _log(rng, 1, 64), "n": _log(rng, 16, 30000),
+           "k": _log(rng, 33, 16384), "group": rng.choice([32, 64, 128]), "zeros": rng.random() < 0.5,
+           "bias": rng.random() < 0.5}
+      if c["n"] * c["k"] <= 28672 * 8192 and c["m"] * c["n"] * c["k"] <= 28672 * 8192 * 16:
+        return c
+  dtype = rng.choice(["f32", "f16", "bf16", "bf16"])
+  cache = rng.choice([dtype, "e4m3"]) if dtype != "f32" else dtype
+  hkv = rng.choice([1, 2, 3, 4, 5, 8, 12, 16])
+  c = {"op": op, "dtype": dtype, "cache": cache, "hq": hkv * rng.choice([1, 1, 2, 3, 4, 6, 8, 16, 24]), "hkv": hkv,
+       "d": rng.choice([32, 64, 80, 96, 128, 128, 192, 256]), "page": rng.choice([16, 32, 48, 64, 128, 256])}
+  if op == "append":
+    c["seqs"] = _log(rng, 1, 256)
+    c["new"] = 1 if rng.random() < 0.4 else _log(rng, 1, 4000)
+    row = 2 * c["hkv"] + c["hq"]
+    while c["seqs"] * c["new"] * row * c["d"] > 7 * 1601 * 48 * 128:
+      c["seqs"] = max(1, c["seqs"] // 2)
+      c["new"] = max(1, c["new"] // 2)
+    c["past"] = rng.choice([0, _log(rng, 1, 200000)])
+    c["rot"] = rng.choice([0, 16, c["d"] // 32 * 16, c["d"], c["d"]])
+    c["interleaved"] = rng.random() < 0.5
+    return c
+  c["seqs"], c["len"] = _log(rng, 1, 256), _log(rng, 1, 131072)
+  while c["seqs"] * c["len"] * max(c["hkv"] * c["d"], c["hq"] * 16) * _BYTES[cache] > 64 * 4096 * 8 * 128 * 2:
+    c["seqs"] = max(1, c["seqs"] // 2)
+    if c["seqs"] == 1:
+      c["len"] = max(1, c["len"] * 3 // 4)
+  c["window"] = rng.choice([0, 0, _log(rng, 1, c["len"])])
+  return c
+
+
+def _ragged(case, most):
+  """The lengths of a case's sequences: the longest first, the others spread below it, and an empty one in larger batches."""
+  r = random.Random("%s %d %d" % (case["op"], case["seqs"], most))
+  lens = [most] + [r.randint(max(1, most // 8), most) for _ in range(case["seqs"] - 1)]
+  if len(lens) > 8:
+    lens[3] = 0
+  return lens
+
+
+def _appended(case):
+  """(tokens already there, new tokens) of every sequence of an append case."""
+  r = random.Random("past %d %d" % (case["seqs"], case["past"]))
+  past = [case["past"]] + [r.randint(0, case["past"]) for _ in range(case["seqs"] - 1)]
+  return past, [1] * case["seqs"] if case["new"] == 1 else _ragged(case, case["new"])
+
+
+def _normal(gen, *shape, dtype="f32", std=1.0):
+  return (torch.randn(*shape, generator=gen, device=_DEV) * std).to(_TYPES[dtype])
+
+
+def prepare(case, seed):
+  gen = torch.Generator(device=_DEV).manual_seed(seed)
+  return {"append": _prepare_append, "attend": _prepare_attend, "w4": _prepare_w4}[case["op"]](dict(case), gen)
+
+
+def _scales(case, gen):
+  """Per-head scales of an 8-bit cache, or none."""
+  if case["cache"] != "e4m3":
+    return None, None
+  return tuple(torch.rand(case["hkv"], generator=gen, device=_DEV) * 0.02 + 0.01 for _ in range(2))
+
+
+def _keep(s, case):
+  """The cache object a program keeps beside the pages."""
+  if own:
+    from tacotron_amd.paged import PagedCache
+    s["handle"] = PagedCache.from_tensors(s["k_pages"], s["v_pages"], k_scale=s["k_scale"], v_scale=s["v_scale"])
+  return s
+
+
+def _prepare_append(case, gen):
+  past, new = _appended(case)
+  page, hkv, hq, d = case["page"], case["hkv"], case["hq"], case["d"]
+  width = max((p + n + page - 1) // page for p, n in zip(past, new)) + 1
+  first = [p // page for p in past]
+  need = [(p + n + page - 1) // page - f for p, n, f in zip(past, new, first)]
+  n_pages = sum(need) + 3
+  order = torch.randperm(n_pages, generator=gen, device=_DEV).to(torch.int32)
+  table = torch.full((case["seqs"], width), int(order[0]), dtype=torch.int32, device=_DEV)   # a prefix nobody writes to
+  at = 1
+  for b in range(case["seqs"]):
+    table[b, first[b]:first[b] + need[b]] = order[at:at + need[b]]
+    at += need[b]
+  tokens = sum(new)
+  s = {"case": case, "table": table}
+  s["k_scale"], s["v_scale"] = _scales(case, gen)
+  for name in ("k", "v"):     # heads outside tokens within a page, as the framework lays its own caches out
+    s[name + "_pages"] = _normal(gen, n_pages, hkv, page, d, dtype=case["cache"]).transpose(1, 2)
+    s[name] = _normal(gen, tokens, hkv, d, dtype=case["dtype"])
+  s["q"] = _normal(gen, tokens, hq, d, dtype=case["dtype"])
+  s["past"] = torch.tensor(past, dtype=torch.int32, device=_DEV)
+  offsets = torch.tensor([0] + new, dtype=torch.int64).cumsum(0)
+  s["offsets"] = None if case["new"] == 1 else offsets.to(torch.int32).to(_DEV)
+  half = case["rot"] // 2
+  s["inv_freq"] = None if not half else 10000.0 ** (-torch.arange(half, dtype=torch.float64, device=_DEV) / half)
+  return _keep(s, case)
+
+
+def _prepare_attend(case, gen):
+  lens = _ragged(case, case["len"])
+  page, hkv, d = case["page"], case["hkv"], case["d"]
+  need = [(n + page - 1) // page for n in lens]
+  width = max(need)
+  n_pages = sum(need) + 2
+  order = torch.randperm(n_pages, generator=gen, device=_DEV).to(torch.int32)
+  table = torch.zeros(case["seqs"], width, dtype=torch.int32, device=_DEV)
+  s = {"case": case}
+  s["k_scale"], s["v_scale"] = _scales(case, gen)
+  for name, std in (("k", 1.0), ("v", 1.0)):
+    unit = 0.02 if case["cache"] == "e4m3" else 1.0
+    pages = torch.empty(n_pages, hkv, page, d, dtype=_TYPES[case["cache"]], device=_DEV)
+    step = max(1, (1 << 27) // (hkv * page * d))
+    for i in range(0, n_pages, step):
+      pages[i:i + step] = _normal(gen, min(step, n_pages - i), hkv, page, d, dtype=case["cache"], std=std / unit)
+    s[name + "_pages"] = pages.transpose(1, 2)
+  at = 0
+  for b, n in enumerate(need):
+    table[b, :n] = order[at:at + n]
+    at += n
+    if lens[b] % page:            # leftovers behind a sequence's end
+      s["k_pages"][table[b, n - 1].long(), lens[b] % page:] = float("nan")
+      s["v_pages"][table[b, n - 1].long(), lens[b] % page:] = float("nan")
+  s["table"] = table
+  s["lens"] = torch.tensor(lens, dtype=torch.int32, device=_DEV)
+  s["q"] = _normal(gen, case["seqs"], case["hq"], d, dtype=case["dtype"], std=1.5)
+  s["scale"] = 1.0 / math.sqrt(d)
+  return _keep(s, case)
+
+
+def _prepare_w4(case, gen):
+  n, k, g = case["n"], case["k"], case["group"]
+  groups = (k + g - 1) // g
+  # codes of normally distributed weights: 4 bits, the middle ones most often
+  codes = (torch.randn(n, groups * g, generator=gen, device=_DEV) * 2.6 + 8).round().clamp(0, 15).to(torch.uint8)
+  codes[:, k:] = 0
+  s = {"case": case, "packed": codes[:, 0::2] | (codes[:, 1::2] << 4)}
+  s["scales"] = ((torch.rand(n, groups, generator=gen, device=_DEV) + 0.5) * (0.4 / math.sqrt(k))).to(_TYPES[case["scales"]])
+  s["zeros"] = torch.randint(5, 12, (n, groups), generator=gen, device=_DEV, dtype=torch.uint8) if case["zeros"] else None
+  s["bias"] = _normal(gen, n, dtype=case["dtype"]) if case["bias"] else None
+  s["x"] = _normal(gen, case["m"], k, dtype=case["dtype"])
+  if own:
+    from tacotron_amd.w4 import W4Matrix
+    s["handle"] = W4Matrix.from_codes(s["packed"], s["scales"], zeros=s["zeros"], bias=s["bias"], in_features=k)
+  return s
+
+
+def run(state):
+  return {"append": _run_append, "attend": _run_attend, "w4": _run_w4}[state["case"]["op"]](state)
+
+
+def _rotated(x, cos, sin, rot, interleaved):
+  x = x.float()
+  if not rot:
+    return x
+  r, rest = x[..., :rot], x[..., rot:]
+  if interleaved:
+    a, b = r[..., 0::2], r[..., 1::2]
+    r = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+  else:
+    a, b = r[..., :rot // 2], r[..., rot // 2:]
+    r = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+  return torch.cat([r, rest], -1)
+
+
+def _run_append(s):
+  c = s["case"]
+  if own:
+    q = s["handle"].append(s["k"], s["v"], s["table"], s["past"], q=s["q"], offsets=s["offsets"], inv_freq=s["inv_freq"],
+                           interleaved=c["interleaved"])
+    return {"q": q, "k_pages": s["k_pages"], "v_pages": s["v_pages"]}
+  tokens = torch.arange(s["k"].shape[0], device=s["k"].device)
+  if s["offsets"] is None:
+    seq, pos = tokens, s["past"].long()
+  else:
+    seq = (s["offsets"][1:, None] <= tokens[None]).sum(0)
+    pos = s["past"].long()[seq] + tokens - s["offsets"].long()[seq]
+  cos = sin = None
+  if c["rot"]:
+    angle = pos.double()[:, None] * s["inv_freq"]
+    cos, sin = angle.cos().float()[:, None], angle.sin().float()[:, None]
+  pages, slots = s["table"][seq, pos // c["page"]].long(), pos % c["page"]
+  for name, x in (("k", _rotated(s["k"], cos, sin, c["rot"], c["interleaved"])), ("v", s["v"].float())):
+    if c["cache"] == "e4m3":
+      x = (x / s[name + "_scale"][:, None]).clamp(-448, 448)
+    s[name + "_pages"][pages, slots] = x.to(_TYPES[c["cache"]])
+  q = _rotated(s["q"], cos, sin, c["rot"], c["interleaved"]).to(s["q"].dtype)
+  return {"q": q, "k_pages": s["k_pages"], "v_pages": s["v_pages"]}
+
+
+def _run_attend(s):
+  c = s["case"]
+  if own:
+    return s["handle"].attend(s["q"], s["table"], s["lens"], scale=s["scale"], window=c["window"], return_lse=True)
+  n, hkv, d = c["seqs"], c["hkv"], c["d"]
+  lens = s["lens"][:, None]
+  pos = torch.arange(s["table"].shape[1] * c["page"], device=s["q"].device)[None]
+  seen = pos < lens
+  if c["window"]:
+    seen = seen & (pos >= lens - c["window"])
+  k = s["k_pages"][s["table"].long()].flatten(1, 2).float()
+  v = s["v_pages"][s["table"].long()].flatten(1, 2).float()
+  if c["cache"] == "e4m3":
+    k, v = k * s["k_scale"][:, None], v * s["v_scale"][:, None]
+  v = torch.where(seen[:, :, None, None], v, 0.0).transpose(1, 2).contiguous()
+  q = s["q"].float().view(n, hkv, c["hq"] // hkv, d)
+  score = torch.matmul(q, k.permute(0, 2, 3, 1).contiguous()) * s["scale"]
+  score = torch.where(seen[:, None, None], score, -math.inf)
+  top = score.amax(-1, keepdim=True)
+  top = torch.where(top == -math.inf, 0.0, top)
+  p = torch.exp(score - top)
+  total = p.sum(-1, keepdim=True)
+  out = torch.matmul(p, v) / torch.where(total == 0, 1.0, total)
+  return out.reshape(n, c["hq"], d).to(s["q"].dtype), (top + torch.log(total)).reshape(n, c["hq"])
+
+
+def _run_w4(s):
+  if own:
+    return s["handle"].matvec(s["x"])
+  c = s["case"]
+  codes = torch.stack([s["packed"] & 15, s["packed"] >> 4], -1).flatten(1).float()
+  n, groups = s["scales"].shape
+  zeros = 8.0 if s["zeros"] is None else s["zeros"].float()[:, :, None]
+  w = ((codes.view(n, groups, c["group"]) - zeros) * s["scales"].float()[:, :, None]).flatten(1)[:, :c["k"]]
+  y = torch.matmul(s["x"].float(), w.t())
+  if s["bias"] is not None:
+    y = y + s["bias"].float()
+  return y.to(s["x"].dtype)
+
+
+def work(case):
+  if case["op"] == "w4":
+    groups = (case["k"] + case["group"] - 1) // case["group"]
+    size = _BYTES[case["dtype"]]
+    read = case["n"] * (case["k"] / 2 + groups * (_BYTES[case["scales"]] + (0.5 if case["zeros"] else 0)))
+    read += (case["m"] * case["k"] + (case["n"] if case["bias"] else 0)) * size
+    return {"bytes": read + case["m"] * case["n"] * size, "flops": 2.0 * case["m"] * case["n"] * case["k"]}
+  size, held, row = _BYTES[case["dtype"]], _BYTES[case["cache"]], case["hkv"] * case["d"]
+  if case["op"] == "append":
+    tokens = sum(_appended(case)[1])
+    return {"bytes": float(tokens * (2 * row * (size + held) + 2 * case["hq"] * case["d"] * size)),
+            "flops": 3.0 * tokens * (case["hkv"] + case["hq"]) * case["rot"]}
+  seen = [min(n, case["window"]) if case["window"] else n for n in _ragged(case, case["len"])]
+  pages = sum(-(-n // case["page"]) for n in seen)
+  return {"bytes": float(sum(seen) * 2 * row * held + case["seqs"] * case["hq"] * (2 * case["d"] * size + 4) + 4 * pages),
+          "flops": 4.0 * sum(seen) * case["hq"] * case["d"]}
+
+
+def exact(case, seed):
+  s = prepare(case, seed)
+  return {"append": _exact_append, "attend": _exact_attend, "w4": _exact_w4}[case["op"]](s, case)
+
+
+def _exact_append(s, c):
+  k_pages, v_pages = s["k_pages"].double().clone(), s["v_pages"].double().clone()
+  q = s["q"].double().clone()
+  past, new = _appended(c)
+  half, at = c["rot"] // 2, 0
+  for b in range(c["seqs"]):
+    rows, pos = slice(at, at + new[b]), torch.arange(past[b], past[b] + new[b], device=_DEV)
+    at += new[b]
+    if not new[b]:
+      continue
+    k, v = s["k"][rows].double(), s["v"][rows].double()
+    if half:
+      turn = torch.polar(torch.ones(new[b], half, dtype=torch.float64, device=_DEV), pos.double()[:, None] * s["inv_freq"])
+      for x in (k, q[rows]):      # rotation as a product of complex numbers
+        first = x[..., 0:c["rot"]:2] if c["interleaved"] else x[..., :half]
+        second = x[..., 1:c["rot"]:2] if c["interleaved"] else x[..., half:c["rot"]]
+        z = torch.complex(first.contiguous(), second.contiguous()) * turn[:, None]
+        first.copy_(z.real)
+        second.copy_(z.imag)
+    if c["cache"] == "e4m3":
+      k = (k / s["k_scale"].double()[:, None]).clamp(-448, 448)
+      v = (v / s["v_scale"].double()[:, None]).clamp(-448, 448)
+    page = s["table"][b].long()[pos // c["page"]]
+    k_pages[page, pos % c["page"]] = k
+    v_pages[page, pos % c["page"]] = v
+  return {"q": q, "k_pages": k_pages, "v_pages": v_pages}
+
+
+def _exact_attend(s, c):
+  out = torch.zeros(c["seqs"], c["hq"], c["d"], dtype=torch.float64, device=_DEV)
+  lse = torch.full((c["seqs"], c["hq"]), -math.inf, dtype=torch.float64, device=_DEV)
+  group = c["hq"] // c["hkv"]
+  for b, n in enumerate(_ragged(c, c["len"])):
+    low = max(0, n - c["window"]) if c["window"] else 0
+    if n == low:
+      continue
+    pos = torch.arange(low, n, device=_DEV)
+    page = s["table"][b].long()[pos // c["page"]]
+    for h in range(c["hkv"]):
+      k, v = s["k_pages"][page, pos % c["page"], h].double(), s["v_pages"][page, pos % c["page"], h].double()
+      if c["cache"] == "e4m3":
+        k, v = k * s["k_scale"][h].double(), v * s["v_scale"][h].double()
+      rows = slice(h * group, (h + 1) * group)
+      score = (s["q"][b, rows].double() @ k.t()) * s["scale"]
+      lse[b, rows] = torch.logsumexp(score, 1)
+      out[b, rows] = torch.softmax(score, 1) @ v
+  return out, lse
+
+
+def _exact_w4(s, c):
+  y = torch.zeros(c["m"], c["n"], dtype=torch.float64, device=_DEV)
+  x, k = s["x"].double(), c["k"]
+  for i in range(0, k, c["group"]):
+    j = min(k, i + c["group"])
+    code = s["packed"][:, i // 2:(i + c["group"]) // 2].long()
+    code = torch.stack([code % 16, code // 16], 2).reshape(c["n"], c["group"])[:, :j - i].double()
+    zero = 8 if s["zeros"] is None else s["zeros"][:, i // c["group"], None].double()
+    y += x[:, i:j] @ ((code - zero) * s["scales"][:, i // c["group"], None].double()).t()
+  return y if s["bias"] is None else y + s["bias"].double()
