@@ -250,6 +250,93 @@ int taco_set_frame_clock(taco_handle h, uint64_t* ticks, int32_t capacity);
 #define TACO_PRECISION_BF16 1
 int taco_set_precision(taco_handle h, int32_t precision);
 
+/* ---- The step of a decoder with self-attention ------------------------------------------------------------------
+ * Operators next to the stages above, for a model whose decoder keeps keys and values of its earlier frames instead of
+ * an LSTM state: a paged cache that takes the new frames of many utterances (taco_kv_append), the attention of one new
+ * frame per utterance over it (taco_kv_attend), and matrix-vector products with 4-bit step weights (taco_qmat_multiply).
+ * They have no counterpart in the reference, whose decoder step is src/tacotron/model.py:454-491.  They need no handle:
+ * every buffer is the caller's, no call allocates, copies or waits (taco_kv_status excepted), so all of them may be
+ * captured into a graph, and calls on different streams may overlap as long as they share no buffer that one of them
+ * writes (a workspace is such a buffer).  `device` is the GPU that all pointers of a call belong to. */
+#define TACO_F32 0
+#define TACO_F16 1
+#define TACO_BF16 2
+#define TACO_E4M3 3           /* 8-bit floats of 3 mantissa bits (OCP), a cache's type only */
+
+/* A cache of n_pages pages of page_size tokens.  Element (page, slot, head, i) of k is at
+ * k[page * k_stride[0] + slot * k_stride[1] + head * k_stride[2] + i]; all strides are in elements, the addresses of all
+ * rows multiples of 16 bytes.  The pages of an utterance are listed in a table: token t of utterance b is in slot
+ * t % page_size of page table[b * table_stride + t / page_size].  page_size and head_dim are multiples of 16 (the
+ * attention reads 16 tokens of a page at a time), head_dim at most 256. */
+typedef struct taco_kv_cache {
+  void* k;
+  void* v;
+  int64_t k_stride[3];        /* page, slot, head */
+  int64_t v_stride[3];
+  const float* k_scale;       /* TACO_E4M3: [n_heads], what a stored 1.0 of that head stands for; NULL otherwise */
+  const float* v_scale;
+  uint32_t* flags;            /* [1], zero at first: what the calls found wrong (taco_kv_status) */
+  int32_t n_pages, page_size, n_heads, head_dim;
+  int32_t dtype;              /* TACO_F32 .. TACO_E4M3 */
+  int32_t device;
+} taco_kv_cache;
+
+typedef struct taco_kv_append_args {
+  const void* k;              /* [n_tokens, n_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
+  const void* v;
+  const void* q;              /* [n_tokens, n_q_heads, head_dim] or NULL */
+  void* q_out;                /* like q (may be q itself); NULL when q is */
+  const int32_t* table;       /* [n_seqs, table_width] */
+  const int32_t* past;        /* [n_seqs] tokens of each utterance that the cache holds already */
+  const int32_t* offsets;     /* [n_seqs + 1], rising: rows offsets[b] .. offsets[b+1]-1 are utterance b's new tokens;
+                                 NULL = one new token each (n_tokens == n_seqs) */
+  const double* inv_freq;     /* [rot_dim / 2] or NULL (rot_dim 0) */
+  int64_t k_stride[2], v_stride[2], q_stride[2], q_out_stride[2];    /* token, head */
+  int64_t table_stride;
+  int32_t n_tokens, n_seqs, table_width, n_q_heads;
+  int32_t rot_dim;            /* how much of a head is rotated: a multiple of 16, 0 .. head_dim */
+  int32_t interleaved;        /* the pairs are (2i, 2i+1) instead of (i, i + rot_dim/2) */
+  int32_t dtype;              /* of k, v, q, q_out: the cache's; TACO_F16 or TACO_BF16 for a TACO_E4M3 cache */
+} taco_kv_append_args;
+
+/* Appends keys and values and rotates keys and queries by their positions on the way: row offsets[b] + j is token
+ * p = past[b] + j of utterance b; with c + is = exp(i * p * inv_freq[n]) (the angle in 64 bits) pair n (x, y) becomes
+ * (x c - y s, y c + x s), in fp32, rounded once to the cache's type - for TACO_E4M3 after the division by the head's
+ * scale, what is beyond +-448 becoming +-448.  Rows in front of offsets[0] or behind offsets[n_seqs] are left alone in
+ * q_out.  A token whose page is not in the table, or whose table entry is no page, is not written and sets a flag.  No two
+ * tokens of a call may have the same place (what is stored there is undefined then). */
+int taco_kv_append(const taco_kv_cache* cache, const taco_kv_append_args* args, void* stream);
+
+typedef struct taco_kv_attend_args {
+  const void* q;              /* [n_seqs, n_q_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
+  void* out;                  /* like q */
+  float* lse;                 /* [n_seqs, n_q_heads] or NULL */
+  const int32_t* table;       /* [n_seqs, table_width] */
+  const int32_t* lens;        /* [n_seqs] tokens of each utterance, the new one included */
+  void* workspace;            /* taco_kv_attend_workspace() bytes, 16-byte aligned; its contents do not matter */
+  int64_t workspace_bytes;
+  int64_t q_stride[2], out_stride[2];     /* utterance, head */
+  int64_t table_stride;
+  float scale;                /* factor of the scores */
+  int32_t window;             /* > 0: only the last `window` tokens are seen; 0: all */
+  int32_t n_seqs, table_width, n_q_heads;
+  int32_t dtype;              /* of q and out: the cache's; TACO_F16 or TACO_BF16 for a TACO_E4M3 cache */
+} taco_kv_attend_args;
+
+/* Attention of one new token per utterance: out = sum_t w_t v_t, w = softmax over the seen tokens of scale * (q . k_t);
+ * query head h reads cache head h / (n_q_heads / n_heads).  lse gets the natural logarithm of the softmax's sum.  An
+ * utterance without seen tokens (length 0, or none left by bad table entries, which set a flag) gets zeros and -inf.
+ * Slots at and behind lens[b] may hold anything.  Statistics and sums are fp32; results do not depend on timing. */
+int taco_kv_attend(const taco_kv_cache* cache, const taco_kv_attend_args* args, void* stream);
+
+/* Bytes of workspace that taco_kv_attend needs for these arguments (its pointers are not looked at), or a negative code.
+ * They depend on the sizes only, not on the lengths. */
+int64_t taco_kv_attend_workspace(const taco_kv_cache* cache, const taco_kv_attend_args* args);
+
+/* Waits for the work enqueued on `stream`, reads and clears the cache's flags: TACO_ERANGE when a call has met a table
+ * entry that is no page, or a position or length outside the table. */
+int taco_kv_status(const taco_kv_cache* cache, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ EXPORTED_SYMBOLS = (
   "taco_last_error", "taco_version", "taco_create", "taco_destroy", "taco_step_weight_bytes",
   "taco_encode", "taco_encode_status", "taco_decode", "taco_decode_resumable", "taco_postnet", "taco_postnet_noalloc", "taco_last_decode_timing",
   "taco_set_frame_clock", "taco_set_precision",
+  "taco_kv_append", "taco_kv_attend", "taco_kv_attend_workspace", "taco_kv_status",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -68,6 +69,11 @@ def lib() -> C.CDLL:
   L.taco_last_decode_timing.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(i32)]
   L.taco_set_frame_clock.argtypes = [vp, vp, i32]
   L.taco_set_precision.argtypes = [vp, i32]
+  L.taco_kv_append.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAppendArgs), vp]
+  L.taco_kv_attend.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAttendArgs), vp]
+  L.taco_kv_attend_workspace.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAttendArgs)]
+  L.taco_kv_attend_workspace.restype = C.c_int64
+  L.taco_kv_status.argtypes = [C.POINTER(abi.TacoKvCache), vp]
   _lib = L
   return L
 

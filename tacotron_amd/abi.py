@@ -57,6 +57,34 @@ class TacoWeights(C.Structure):
   ]
 
 
+# Element types of the self-attention step's operators.
+TACO_F32, TACO_F16, TACO_BF16, TACO_E4M3 = 0, 1, 2, 3
+DTYPES = {torch.float32: TACO_F32, torch.float16: TACO_F16, torch.bfloat16: TACO_BF16, torch.float8_e4m3fn: TACO_E4M3}
+
+
+class TacoKvCache(C.Structure):
+  _fields_ = [
+    ("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+    ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("flags", C.c_void_p),
+    ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_heads", C.c_int32), ("head_dim", C.c_int32),
+    ("dtype", C.c_int32), ("device", C.c_int32),
+  ]
+
+
+class TacoKvAppendArgs(C.Structure):
+  _fields_ = [(n, C.c_void_p) for n in ("k", "v", "q", "q_out", "table", "past", "offsets", "inv_freq")] + [
+    ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2), ("q_stride", C.c_int64 * 2), ("q_out_stride", C.c_int64 * 2),
+    ("table_stride", C.c_int64),
+  ] + [(n, C.c_int32) for n in ("n_tokens", "n_seqs", "table_width", "n_q_heads", "rot_dim", "interleaved", "dtype")]
+
+
+class TacoKvAttendArgs(C.Structure):
+  _fields_ = [(n, C.c_void_p) for n in ("q", "out", "lse", "table", "lens", "workspace")] + [
+    ("workspace_bytes", C.c_int64), ("q_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2), ("table_stride", C.c_int64),
+    ("scale", C.c_float),
+  ] + [(n, C.c_int32) for n in ("window", "n_seqs", "table_width", "n_q_heads", "dtype")]
+
+
 def build_dims(hp: HParams, n_symbols: int, n_stresses: Optional[int], n_speakers: Optional[int],
                n_tones: Optional[int], n_durations: Optional[int]) -> Tuple[TacoDims, ModelDims]:
   md = model_dims(hp, n_symbols, n_stresses, n_speakers, n_tones, n_durations)

@@ -76,19 +76,6 @@ int ensure_floats(float** p, size_t* have, size_t want) {
   return TACO_OK;
 }
 
-// Makes the handle's device current for the duration of an entry point and gives the caller its own back.
-struct DeviceScope {
-  int prev = -1;
-  hipError_t status;
-  explicit DeviceScope(int device) {
-    (void)hipGetDevice(&prev);
-    status = hipSetDevice(device);
-  }
-  ~DeviceScope() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
-
 }  // namespace
 
 extern "C" int taco_create(const taco_dims* dims, const taco_weights* weights, int device, taco_handle* out) {

@@ -19,6 +19,19 @@ void taco_set_error(const char* fmt, ...);
     if (e_ != hipSuccess) TACO_FAIL(TACO_EHIP, "%s failed: %s", #call, hipGetErrorString(e_)); \
   } while (0)
 
+// Makes a device current for the duration of an entry point and gives the caller its own back.
+struct DeviceScope {
+  int prev = -1;
+  hipError_t status;
+  explicit DeviceScope(int device) {
+    (void)hipGetDevice(&prev);
+    status = hipSetDevice(device);
+  }
+  ~DeviceScope() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
 // ---- compile-time capacities of the persistent decoder ----------------------------------------
 // LSTM rows live in registers in chunks of 256 columns (one ds_read_b128 per lane per chunk).
 constexpr int TACO_CHUNK = 256;
@@ -150,6 +163,9 @@ struct taco_handle_s {
   unsigned long long* frame_clock;   // caller's device buffer for per-frame clock readings, or NULL
   int frame_clock_cap;
 };
+
+// What the entry points without a handle know of a device: 0 for a gfx950 GPU and its number of CUs, else an error code.
+int taco_device_check(int device, int* n_cu);
 
 // ---- launchers implemented in the kernel translation units ----------------------------------
 int taco_launch_embed(taco_handle h, const int64_t* const* ids_dev, const int32_t* lens, int B, int T,

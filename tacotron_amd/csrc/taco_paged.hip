@@ -1,0 +1,603 @@
+// A paged cache of keys and values and the attention of one new token over it (taco_kv_* in include/taco.h): the step of
+// a decoder with self-attention.  Both kernels move every byte of their operands once and are bound by that.
+#include "taco_place.h"
+#include "taco_step.h"
+
+#include <atomic>
+
+namespace {
+
+// ---- append ---------------------------------------------------------------------------------------------------------
+
+struct AppendParams {
+  const char *k, *v, *q;
+  char *q_out, *k_pages, *v_pages;
+  int64_t k_st[2], v_st[2], q_st[2], qo_st[2], kp_st[3], vp_st[3];   // bytes
+  const float *k_scale, *v_scale;
+  const int32_t *table, *past, *offsets;
+  const double* inv_freq;
+  uint32_t* flags;
+  int64_t table_stride;
+  taco_divisor page;
+  int32_t n_tokens, n_seqs, table_width, n_pages, n_heads, n_q_heads, head_dim, rot_dim, interleaved;
+};
+
+// sin and cos of pos * freq.  The angle is reduced in 64 bits (fp32 would lose an angle of 1e5 rad to 8e-3), the rest
+// |r| <= pi/4 goes through the Taylor polynomials of degree 9 and 10, whose first omitted terms are 1.8e-9 and 1.2e-10.
+__device__ __forceinline__ void sin_cos(double angle, float& s, float& c) {
+  const double n = rint(angle * 0.63661977236758134308);            // 2 / pi
+  double r = fma(-n, 1.57079632679489655800, angle);                // pi / 2 in two parts
+  r = fma(-n, 6.12323399573676603587e-17, r);
+  const float x = (float)r, z = x * x;
+  const float ps = x + x * z * (-1.0f / 6 + z * (1.0f / 120 + z * (-1.0f / 5040 + z * (1.0f / 362880))));
+  const float pc = 1.0f + z * (-0.5f + z * (1.0f / 24 + z * (-1.0f / 720 + z * (1.0f / 40320 + z * (-1.0f / 3628800)))));
+  const int quadrant = (int)(long long)n & 3;
+  s = (quadrant & 1) ? pc : ps;
+  c = (quadrant & 1) ? ps : pc;
+  if (quadrant & 2) s = -s;
+  if (quadrant == 1 || quadrant == 2) c = -c;
+}
+
+// Rounds to the cache's type: 8-bit caches hold x / scale, held inside the type's range (a NaN stays one).
+template <int C>
+__device__ __forceinline__ void store_cache(char* p, float (&x)[8], float scale) {
+  if constexpr (C == TACO_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = x[i] / scale;
+      x[i] = y != y ? y : __builtin_amdgcn_fmed3f(y, -448.0f, 448.0f);
+    }
+  }
+  taco_store8<C>(p, x);
+}
+
+// One workgroup per token.  Its first rot_dim / 2 threads compute the token's sines and cosines once for all heads; then
+// every thread takes pieces of 16 elements of a head: both halves of 8 pairs, or 16 elements that are only copied.
+template <int T, int C>
+__global__ __launch_bounds__(256) void taco_kv_append_kernel(const AppendParams a) {
+  __shared__ float cs[128], sn[128];
+  const int n = blockIdx.x, tid = threadIdx.x;
+  int b = n, j = 0;
+  if (a.offsets) {
+    // the utterance: how many of offsets[1 .. n_seqs] are at or below this row (64 at a time, every wave for itself)
+    b = 0;
+    for (int i = 0; i < a.n_seqs; i += 64) {
+      const int at = i + (tid & 63);
+      b += __popcll(__ballot(at < a.n_seqs && a.offsets[at + 1] <= n));
+    }
+    if (b >= a.n_seqs) return;              // behind the last utterance
+    j = n - a.offsets[b];
+    if (j < 0) return;                      // in front of the first
+  }
+  const int past = a.past[b];
+  const int64_t pos = (int64_t)past + j;
+  const taco_place place = taco_find(a.table + (int64_t)b * a.table_stride, a.table_width, a.n_pages, pos, a.page);
+  if (place.flag && tid == 0) atomicOr(a.flags, place.flag);
+  const int64_t page = place.page, slot = place.unit;
+  const int half = a.rot_dim / 2;
+  if (tid < half) {
+    float s, c;
+    sin_cos((double)pos * a.inv_freq[tid], s, c);
+    sn[tid] = s;
+    cs[tid] = c;
+  }
+  __syncthreads();
+
+  constexpr int TB = taco_size_of<T>, CB = taco_size_of<C>;
+  const int per_head = a.head_dim / 16, rotated = a.rot_dim / 16;
+  const int heads = (a.q ? a.n_q_heads : 0) + 2 * a.n_heads;
+  for (int i = tid; i < heads * per_head; i += 256) {
+    const int head = i / per_head, piece = i % per_head;
+    // heads of k, then v, then q
+    const bool is_k = head < a.n_heads, is_v = !is_k && head < 2 * a.n_heads;
+    const int h = is_k ? head : is_v ? head - a.n_heads : head - 2 * a.n_heads;
+    if ((is_k || is_v) && page < 0) continue;
+    const bool turn = !is_v && piece < rotated;
+    const bool split = turn && !a.interleaved;
+    const int e0 = split ? piece * 8 : piece * 16, e1 = split ? half + piece * 8 : piece * 16 + 8;
+    const char* src = is_k ? a.k + n * a.k_st[0] + h * a.k_st[1]
+                    : is_v ? a.v + n * a.v_st[0] + h * a.v_st[1] : a.q + n * a.q_st[0] + h * a.q_st[1];
+    float x[8], y[8];
+    taco_load8<T>(src + e0 * TB, x);
+    taco_load8<T>(src + e1 * TB, y);
+    if (turn) {
+      const float *c = cs + piece * 8, *s = sn + piece * 8;
+      if (split) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float u = x[e], w = y[e];
+          x[e] = u * c[e] - w * s[e];
+          y[e] = w * c[e] + u * s[e];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float u = x[2 * e], w = x[2 * e + 1];
+          x[2 * e] = u * c[e] - w * s[e];
+          x[2 * e + 1] = w * c[e] + u * s[e];
+          const float u2 = y[2 * e], w2 = y[2 * e + 1];
+          y[2 * e] = u2 * c[4 + e] - w2 * s[4 + e];
+          y[2 * e + 1] = w2 * c[4 + e] + u2 * s[4 + e];
+        }
+      }
+    }
+    if (is_k || is_v) {
+      char* dst = is_k ? a.k_pages + page * a.kp_st[0] + slot * a.kp_st[1] + h * a.kp_st[2]
+                       : a.v_pages + page * a.vp_st[0] + slot * a.vp_st[1] + h * a.vp_st[2];
+      const float scale = C == TACO_E4M3 ? (is_k ? a.k_scale[h] : a.v_scale[h]) : 1.0f;
+      store_cache<C>(dst + e0 * CB, x, scale);
+      store_cache<C>(dst + e1 * CB, y, scale);
+    } else {
+      char* dst = a.q_out + n * a.qo_st[0] + h * a.qo_st[1];
+      taco_store8<T>(dst + e0 * TB, x);
+      taco_store8<T>(dst + e1 * TB, y);
+    }
+  }
+}
+
+// ---- attend ---------------------------------------------------------------------------------------------------------
+
+struct AttendParams {
+  const char *k_pages, *v_pages, *q;
+  char* out;
+  float* lse;
+  int64_t kp_st[3], vp_st[3], q_st[2], o_st[2];      // bytes
+  const float *k_scale, *v_scale;
+  const int32_t *table, *lens;
+  uint32_t* flags;
+  int64_t table_stride;
+  taco_divisor page16;                                    // 16-token blocks of a page
+  float scale_log2;                                  // scale * log2(e)
+  int32_t n_seqs, table_width, n_pages, n_heads, n_q_heads, group, q_tiles, head_dim, window;
+};
+
+constexpr int AT_WAVES = 4;
+constexpr float NEG_INF = -__builtin_inff();
+
+// What a wave holds of one (utterance, cache head, up to 16 query heads): the running maximum and sum of the softmax of
+// query column l & 15 (base 2; the sum is this lane's own part of it) and the unnormalised output, transposed:
+// o[blk][e][i] belongs to element blk * 16 * VE + (4 * (l >> 4) + i) * VE + e of that query's head.
+template <int NB, int VE>
+struct State {
+  float m = NEG_INF, l = 0.0f;
+  taco_f4 o[NB][VE];
+};
+
+// The attention works on tiles of TT tokens per wave (32 of 16- and 8-bit elements, 16 of fp32), straight from memory into
+// the matrix cores' operand layout, so that nothing of the cache passes through LDS:
+//   scores, transposed:  S^T[token][query] = K Q^T.  Lane l holds 16 bytes of row token l & 15 (contraction over head_dim).
+//   output, transposed:  O^T[element][query] += V^T P^T.  The scores' layout - lane l has tokens 4 (l >> 4) + i of column
+//     l & 15 - is the operand layout of P^T with the tokens taken in that order, so weights never change lanes.  A lane
+//     loads VE neighbouring elements of each of its own tokens (16 lanes read one row end to end) and element e of all of
+//     them is one operand: for 16-bit types a v_perm per word turns rows into operands.
+// Weights are rounded to the operand type twice, p = hi + lo: one rounding alone would be as large as that of the
+// output itself, and the second product costs nothing while memory is the bound.
+template <int T, int C, int DP>
+struct Attend {
+  static constexpr int CB = taco_size_of<C>;
+  static constexpr int TT = C == TACO_F32 ? 16 : 32;           // tokens of a tile
+  static constexpr int SUB = TT / 16;
+  static constexpr int KE = 16 / CB;                           // elements of a 16-byte load of K
+  static constexpr int NK = DP * CB / 64;                      // loads per row of K: four lanes read 64 bytes of it
+  static constexpr int NQ = C == TACO_F32 ? DP / 16 : DP / 32; // operands of Q
+  static constexpr int VE = C == TACO_F32 ? 4 : C == TACO_E4M3 ? DP / 16 : (DP < 128 ? DP / 16 : 8);   // elements of a load of V
+  static constexpr int NB = DP / (16 * VE);
+  static constexpr int VW = VE * CB / 4;                       // ... in words
+  using St = State<NB, VE>;
+
+  // Query operands: for the K operand whose lane holds elements d0 .. of a row, the same elements of query column l & 15.
+  static __device__ void load_q(const AttendParams& a, int b, int h, int qt, taco_u4 (&q)[NQ]) {
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const bool have = qt * 16 + col < a.group;
+    const char* row = a.q + (int64_t)b * a.q_st[0] + (int64_t)(h * a.group + qt * 16 + (have ? col : 0)) * a.q_st[1];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      int d;      // first element
+      if constexpr (C == TACO_E4M3) d = (n >> 1) * 64 + g * 16 + (n & 1) * 8;
+      else d = (n * 4 + g) * KE;
+      q[n] = taco_u4{0, 0, 0, 0};
+      if (have && d < a.head_dim) q[n] = *(const taco_u4*)(row + (int64_t)d * taco_size_of<T>);
+    }
+  }
+
+  static __device__ __forceinline__ void tile(const AttendParams& a, int b, int h, int t0, int low, int len, float factor,
+                                              const taco_u4 (&q)[NQ], St& st) {
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    // the pages of the tile's 16-token blocks; a block behind the last token, or on a bad page, reads page 0 and is masked
+    const int32_t* row = a.table + (int64_t)b * a.table_stride;
+    int64_t page[SUB];
+    int slot[SUB];
+    bool ok[SUB];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const int blk = t0 / 16 + s;
+      taco_place place = {-1, 0, 0};
+      if (blk * 16 < len && blk * 16 + 16 > low) place = taco_find(row, a.table_width, a.n_pages, blk, a.page16);
+      if (place.flag && lane == 0) atomicOr(a.flags, place.flag);
+      ok[s] = place.page >= 0;
+      page[s] = ok[s] ? place.page : 0;
+      slot[s] = (int)place.unit * 16;
+    }
+    taco_u4 kr[SUB][NK];
+    uint32_t vr[SUB * 4][NB][VW];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      const char* row = a.k_pages + page[s] * a.kp_st[0] + (int64_t)(slot[s] + col) * a.kp_st[1] + h * a.kp_st[2];
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        const int d = (n * 4 + g) * KE;
+        kr[s][n] = taco_u4{0, 0, 0, 0};
+        if (d < a.head_dim) kr[s][n] = *(const taco_u4*)(row + d * CB);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const char* row = a.v_pages + page[s] * a.vp_st[0] + (int64_t)(slot[s] + g * 4 + i) * a.vp_st[1] + h * a.vp_st[2];
+#pragma unroll
+        for (int blk = 0; blk < NB; ++blk) {
+          const int d = blk * 16 * VE + col * VE;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vr[s * 4 + i][blk][w] = 0;
+          if (d < a.head_dim) {
+            if constexpr (VW == 4) {
+              const taco_u4 x = *(const taco_u4*)(row + d * CB);
+#pragma unroll
+              for (int w = 0; w < 4; ++w) vr[s * 4 + i][blk][w] = x[w];
+            } else if constexpr (VW == 2) {
+              const taco_u2 x = *(const taco_u2*)(row + d * CB);
+              vr[s * 4 + i][blk][0] = x[0];
+              vr[s * 4 + i][blk][1] = x[1];
+            } else {
+              vr[s * 4 + i][blk][0] = *(const uint32_t*)(row + d * CB);
+            }
+          }
+        }
+      }
+    // scores
+    float p[SUB * 4];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      taco_f4 acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < NK; ++n) {
+        if constexpr (C == TACO_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[s][n][e]), __uint_as_float(q[n][e]), acc, 0, 0, 0);
+        } else if constexpr (C == TACO_E4M3) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const taco_u4 x = {widen<0>(kr[s][n][2 * e]), widen<1>(kr[s][n][2 * e]), widen<0>(kr[s][n][2 * e + 1]), widen<1>(kr[s][n][2 * e + 1])};
+            acc = taco_mfma32<T>(x, q[2 * n + e], acc);
+          }
+        } else {
+          acc = taco_mfma32<T>(kr[s][n], q[n], acc);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[s * 4 + i] = acc[i] * factor;
+    }
+    // masked tokens: their weight is 0, and what lies in their V rows must not meet it (0 * NaN)
+    bool whole = t0 >= low && t0 + TT <= len;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) whole = whole && ok[s];
+    if (!whole) {
+#pragma unroll
+      for (int s = 0; s < SUB; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = t0 + s * 16 + g * 4 + i;
+          if (!(ok[s] && t >= low && t < len)) {
+            p[s * 4 + i] = NEG_INF;
+#pragma unroll
+            for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+              for (int w = 0; w < VW; ++w) vr[s * 4 + i][blk][w] = 0;
+          }
+        }
+    }
+    // running maximum; the outputs are rescaled only in the tiles that raise it
+    float top = p[0];
+#pragma unroll
+    for (int i = 1; i < SUB * 4; ++i) top = fmaxf(top, p[i]);
+    top = taco_max_rows(top);
+    if (__any(top > st.m)) {
+      const float m = fmaxf(st.m, top);
+      const float f = m == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
+      st.m = m;
+      st.l *= f;
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) st.o[blk][e] *= f;
+    }
+    const float m = st.m == NEG_INF ? 0.0f : st.m;
+#pragma unroll
+    for (int i = 0; i < SUB * 4; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(p[i] - m);
+      st.l += p[i];
+    }
+    // output
+    if constexpr (C == TACO_F32) {
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st.o[blk][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][blk][e]), p[i], st.o[blk][e], 0, 0, 0);
+    } else {
+      taco_u4 hi, lo;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        hi[w] = taco_pack2<T>(p[2 * w], p[2 * w + 1]);
+        lo[w] = taco_pack2<T>(p[2 * w] - taco_low<T>(hi[w]), p[2 * w + 1] - taco_high<T>(hi[w]));
+      }
+#pragma unroll
+      for (int blk = 0; blk < NB; ++blk)
+#pragma unroll
+        for (int w = 0; w < VE / 2; ++w) {       // elements 2w, 2w + 1
+          uint32_t x[8];
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            if constexpr (C == TACO_E4M3) x[t] = (w & 1) ? widen<1>(vr[t][blk][w / 2]) : widen<0>(vr[t][blk][w / 2]);
+            else x[t] = vr[t][blk][w];
+          }
+          taco_u4 even, odd;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            even[t] = __builtin_amdgcn_perm(x[2 * t + 1], x[2 * t], 0x05040100u);
+            odd[t] = __builtin_amdgcn_perm(x[2 * t + 1], x[2 * t], 0x07060302u);
+          }
+          st.o[blk][2 * w] = taco_mfma32<T>(even, hi, st.o[blk][2 * w]);
+          st.o[blk][2 * w] = taco_mfma32<T>(even, lo, st.o[blk][2 * w]);
+          st.o[blk][2 * w + 1] = taco_mfma32<T>(odd, hi, st.o[blk][2 * w + 1]);
+          st.o[blk][2 * w + 1] = taco_mfma32<T>(odd, lo, st.o[blk][2 * w + 1]);
+        }
+    }
+  }
+
+  // Two 8-bit floats (the low or the high half of a word) as two 16-bit ones; exact in both 16-bit types.
+  template <int HALF>
+  static __device__ __forceinline__ uint32_t widen(uint32_t w) {
+    if constexpr (T == TACO_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, HALF));
+    else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HALF));
+  }
+};
+
+// One workgroup per (utterance, cache head, 16 of its query heads): its waves take the tiles in turn and are joined
+// through LDS.
+template <int T, int C, int DP>
+__global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const AttendParams a) {
+  using A = Attend<T, C, DP>;
+  extern __shared__ float lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const int qt = blockIdx.x % a.q_tiles, bh = blockIdx.x / a.q_tiles, h = bh % a.n_heads, b = bh / a.n_heads;
+  const int rows = min(a.group - qt * 16, 16);
+  int len = a.lens[b];
+  const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
+  if (len < 0 || len > room) {
+    if (threadIdx.x == 0) atomicOr(a.flags, TACO_KV_BAD_PLACE);
+    len = len < 0 ? 0 : (int)room;
+  }
+  const int low = a.window > 0 ? max(0, len - a.window) : 0;
+  taco_u4 q[A::NQ];
+  A::load_q(a, b, h, qt, q);
+  float factor = a.scale_log2;
+  if (C == TACO_E4M3) factor *= a.k_scale[h];
+  typename A::St st;
+#pragma unroll
+  for (int blk = 0; blk < A::NB; ++blk)
+#pragma unroll
+    for (int e = 0; e < A::VE; ++e) st.o[blk][e] = taco_f4{0, 0, 0, 0};
+  for (int t0 = low / A::TT * A::TT + wave * A::TT; t0 < len; t0 += AT_WAVES * A::TT) A::tile(a, b, h, t0, low, len, factor, q, st);
+  // join the waves: [wave][query][m, l, DP outputs]
+  const float l = taco_sum_rows(st.l);
+  float* mine = lds + (wave * rows + col) * (DP + 2);
+  if (col < rows) {
+    if (g == 0) { mine[0] = st.m; mine[1] = l; }
+#pragma unroll
+    for (int blk = 0; blk < A::NB; ++blk)
+#pragma unroll
+      for (int e = 0; e < A::VE; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine[2 + blk * 16 * A::VE + (4 * g + i) * A::VE + e] = st.o[blk][e][i];
+  }
+  __syncthreads();
+  const float v_scale = C == TACO_E4M3 ? a.v_scale[h] : 1.0f;
+  for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
+    const int r = i / DP, d = i % DP;
+    if (d >= a.head_dim) continue;
+    float m = NEG_INF;
+    for (int w = 0; w < AT_WAVES; ++w) m = fmaxf(m, lds[(w * rows + r) * (DP + 2)]);
+    float sum = 0.0f, o = 0.0f;
+    for (int w = 0; w < AT_WAVES; ++w) {
+      const float* p = lds + (w * rows + r) * (DP + 2);
+      const float f = p[0] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
+      sum += f * p[1];
+      o += f * p[2 + d];
+    }
+    const int head = h * a.group + qt * 16 + r;
+    o = sum == 0.0f ? 0.0f : o / sum * v_scale;
+    char* out = a.out + (int64_t)b * a.o_st[0] + (int64_t)head * a.o_st[1];
+    if constexpr (T == TACO_F32) ((float*)out)[d] = o;
+    else if constexpr (T == TACO_BF16) ((__bf16*)out)[d] = (__bf16)o;
+    else ((_Float16*)out)[d] = (_Float16)o;
+    if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------
+
+bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// Addresses of rows: base and strides (elements) in multiples of 16 bytes; writes the strides in bytes.
+template <int N>
+bool row_strides(const void* base, const int64_t* stride, int size, int64_t (&bytes)[N]) {
+  bool ok = base && aligned(base);
+  for (int i = 0; i < N; ++i) {
+    bytes[i] = stride[i] * size;
+    ok = ok && bytes[i] % 16 == 0;
+  }
+  return ok;
+}
+
+int check_cache(const taco_kv_cache* c, const char* who, int dtype) {
+  if (!c) TACO_FAIL(TACO_EINVAL, "%s: NULL cache", who);
+  if (c->dtype < TACO_F32 || c->dtype > TACO_E4M3) TACO_FAIL(TACO_EINVAL, "%s: cache dtype %d", who, c->dtype);
+  if (c->dtype == TACO_E4M3 ? dtype != TACO_F16 && dtype != TACO_BF16 : dtype != c->dtype)
+    TACO_FAIL(TACO_EINVAL, "%s: dtype %d does not go with a cache of dtype %d", who, dtype, c->dtype);
+  if (c->n_pages < 1 || c->n_heads < 1 || c->n_heads > 65535) TACO_FAIL(TACO_EINVAL, "%s: %d pages, %d heads", who, c->n_pages, c->n_heads);
+  if (c->page_size < 16 || c->page_size % 16 || c->page_size > 65536) TACO_FAIL(TACO_EINVAL, "%s: page_size %d is not a multiple of 16 up to 65536", who, c->page_size);
+  if (c->head_dim < 16 || c->head_dim % 16 || c->head_dim > 256) TACO_FAIL(TACO_EINVAL, "%s: head_dim %d is not a multiple of 16 up to 256", who, c->head_dim);
+  if ((c->dtype == TACO_E4M3) != (c->k_scale && c->v_scale) || (c->k_scale == nullptr) != (c->v_scale == nullptr))
+    TACO_FAIL(TACO_EINVAL, "%s: scales belong to 8-bit caches, and those need both", who);
+  if (!c->flags) TACO_FAIL(TACO_EINVAL, "%s: NULL flags", who);
+  return TACO_OK;
+}
+
+}  // namespace
+
+int taco_device_check(int device, int* n_cu) {
+  static std::atomic<int> known[64];       // CUs of a gfx950 device, 0 = not asked yet
+  if (device < 0 || device >= 64) TACO_FAIL(TACO_EINVAL, "device %d", device);
+  int n = known[device].load(std::memory_order_relaxed);
+  if (n == 0) {
+    hipDeviceProp_t prop;
+    TACO_HIP(hipGetDeviceProperties(&prop, device));
+    bool same = true;
+    for (int i = 0; i < 6; ++i) same = same && prop.gcnArchName[i] == "gfx950"[i];
+    if (!same) TACO_FAIL(TACO_EINVAL, "device %d is %s; this library is built for gfx950 only", device, prop.gcnArchName);
+    n = prop.multiProcessorCount;
+    known[device].store(n, std::memory_order_relaxed);
+  }
+  *n_cu = n;
+  return TACO_OK;
+}
+
+extern "C" int taco_kv_append(const taco_kv_cache* c, const taco_kv_append_args* t, void* stream) {
+  const char* who = "taco_kv_append";
+  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
+  int rc = check_cache(c, who, t->dtype);
+  if (rc != TACO_OK) return rc;
+  if (t->n_tokens < 0 || t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d tokens, %d utterances, table width %d", who, t->n_tokens, t->n_seqs, t->table_width);
+  if (!t->offsets && t->n_tokens != t->n_seqs) TACO_FAIL(TACO_EINVAL, "%s: %d tokens for %d utterances without offsets", who, t->n_tokens, t->n_seqs);
+  if (t->rot_dim < 0 || t->rot_dim % 16 || t->rot_dim > c->head_dim) TACO_FAIL(TACO_EINVAL, "%s: rot_dim %d is not a multiple of 16 up to head_dim %d", who, t->rot_dim, c->head_dim);
+  if (t->rot_dim && !t->inv_freq) TACO_FAIL(TACO_EINVAL, "%s: rot_dim %d without frequencies", who, t->rot_dim);
+  if ((t->q == nullptr) != (t->q_out == nullptr) || (t->q && (t->n_q_heads < 1 || t->n_q_heads > 65535))) TACO_FAIL(TACO_EINVAL, "%s: queries", who);
+  if (t->n_tokens == 0 || t->n_seqs == 0) return TACO_OK;
+  if (!t->table || !t->past) TACO_FAIL(TACO_EINVAL, "%s: NULL table or past", who);
+  AppendParams a;
+  const int size = t->dtype == TACO_F32 ? 4 : 2, held = c->dtype == TACO_F32 ? 4 : c->dtype == TACO_E4M3 ? 1 : 2;
+  bool ok = row_strides(t->k, t->k_stride, size, a.k_st) && row_strides(t->v, t->v_stride, size, a.v_st) &&
+            row_strides(c->k, c->k_stride, held, a.kp_st) && row_strides(c->v, c->v_stride, held, a.vp_st);
+  a.q_st[0] = a.q_st[1] = a.qo_st[0] = a.qo_st[1] = 0;
+  if (t->q) ok = ok && row_strides(t->q, t->q_stride, size, a.q_st) && row_strides(t->q_out, t->q_out_stride, size, a.qo_st);
+  if (!ok) TACO_FAIL(TACO_EINVAL, "%s: rows must start at multiples of 16 bytes (and not be NULL)", who);
+  int n_cu;
+  DeviceScope on_device(c->device);
+  TACO_HIP(on_device.status);
+  rc = taco_device_check(c->device, &n_cu);
+  if (rc != TACO_OK) return rc;
+  a.k = (const char*)t->k; a.v = (const char*)t->v; a.q = (const char*)t->q; a.q_out = (char*)t->q_out;
+  a.k_pages = (char*)c->k; a.v_pages = (char*)c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale;
+  a.table = t->table; a.past = t->past; a.offsets = t->offsets; a.inv_freq = t->inv_freq; a.flags = c->flags;
+  a.table_stride = t->table_stride; a.page = taco_make_divisor((uint32_t)c->page_size);
+  a.n_tokens = t->n_tokens; a.n_seqs = t->n_seqs; a.table_width = t->table_width; a.n_pages = c->n_pages;
+  a.n_heads = c->n_heads; a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.rot_dim = t->rot_dim; a.interleaved = t->interleaved;
+  const dim3 grid((unsigned)t->n_tokens), block(256);
+  hipStream_t s = (hipStream_t)stream;
+  if (c->dtype == TACO_F32) taco_kv_append_kernel<TACO_F32, TACO_F32><<<grid, block, 0, s>>>(a);
+  else if (c->dtype == TACO_F16) taco_kv_append_kernel<TACO_F16, TACO_F16><<<grid, block, 0, s>>>(a);
+  else if (c->dtype == TACO_BF16) taco_kv_append_kernel<TACO_BF16, TACO_BF16><<<grid, block, 0, s>>>(a);
+  else if (t->dtype == TACO_F16) taco_kv_append_kernel<TACO_F16, TACO_E4M3><<<grid, block, 0, s>>>(a);
+  else taco_kv_append_kernel<TACO_BF16, TACO_E4M3><<<grid, block, 0, s>>>(a);
+  TACO_HIP(hipGetLastError());
+  return TACO_OK;
+}
+
+extern "C" int64_t taco_kv_attend_workspace(const taco_kv_cache* c, const taco_kv_attend_args* t) {
+  const char* who = "taco_kv_attend_workspace";
+  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
+  const int rc = check_cache(c, who, t->dtype);
+  if (rc != TACO_OK) return rc;
+  return 0;
+}
+
+namespace {
+
+template <int T, int C, int DP>
+int launch_attend(const AttendParams& a, hipStream_t s) {
+  const int rows = a.group < 16 ? a.group : 16;
+  const size_t lds = (size_t)AT_WAVES * rows * (DP + 2) * 4;
+  auto kernel = taco_kv_attend_kernel<T, C, DP>;
+  if (lds > 65536) TACO_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+  kernel<<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles)), dim3(64 * AT_WAVES), lds, s>>>(a);
+  TACO_HIP(hipGetLastError());
+  return TACO_OK;
+}
+template <int T, int C>
+int launch_attend(const AttendParams& a, hipStream_t s) {
+  if (a.head_dim <= 64) return launch_attend<T, C, 64>(a, s);
+  if (a.head_dim <= 128) return launch_attend<T, C, 128>(a, s);
+  return launch_attend<T, C, 256>(a, s);
+}
+
+}  // namespace
+
+extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, void* stream) {
+  const char* who = "taco_kv_attend";
+  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
+  int rc = check_cache(c, who, t->dtype);
+  if (rc != TACO_OK) return rc;
+  if (t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d utterances, table width %d", who, t->n_seqs, t->table_width);
+  if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
+  if (t->window < 0) TACO_FAIL(TACO_EINVAL, "%s: window %d", who, t->window);
+  if (!(t->scale == t->scale) || t->scale - t->scale != 0.0f) TACO_FAIL(TACO_EINVAL, "%s: scale is not finite", who);
+  if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
+  if (t->n_seqs == 0) return TACO_OK;
+  if (!t->lens || (!t->table && t->table_width)) TACO_FAIL(TACO_EINVAL, "%s: NULL table or lens", who);
+  AttendParams a;
+  const int size = t->dtype == TACO_F32 ? 4 : 2, held = c->dtype == TACO_F32 ? 4 : c->dtype == TACO_E4M3 ? 1 : 2;
+  if (!(row_strides(t->q, t->q_stride, size, a.q_st) && row_strides(t->out, t->out_stride, size, a.o_st) &&
+        row_strides(c->k, c->k_stride, held, a.kp_st) && row_strides(c->v, c->v_stride, held, a.vp_st)))
+    TACO_FAIL(TACO_EINVAL, "%s: rows must start at multiples of 16 bytes (and not be NULL)", who);
+  a.group = t->n_q_heads / c->n_heads;
+  a.q_tiles = (a.group + 15) / 16;
+  if ((int64_t)t->n_seqs * c->n_heads * a.q_tiles >= (1ll << 31)) TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads", who, t->n_seqs, t->n_q_heads);
+  int n_cu;
+  DeviceScope on_device(c->device);
+  TACO_HIP(on_device.status);
+  rc = taco_device_check(c->device, &n_cu);
+  if (rc != TACO_OK) return rc;
+  a.k_pages = (const char*)c->k; a.v_pages = (const char*)c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale;
+  a.q = (const char*)t->q; a.out = (char*)t->out; a.lse = t->lse; a.table = t->table; a.lens = t->lens; a.flags = c->flags;
+  a.table_stride = t->table_stride; a.page16 = taco_make_divisor((uint32_t)c->page_size / 16);
+  a.scale_log2 = t->scale * 1.44269504088896340736f;
+  a.n_seqs = t->n_seqs; a.table_width = t->table_width; a.n_pages = c->n_pages; a.n_heads = c->n_heads;
+  a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.window = t->window;
+  hipStream_t s = (hipStream_t)stream;
+  if (c->dtype == TACO_F32) return launch_attend<TACO_F32, TACO_F32>(a, s);
+  if (c->dtype == TACO_F16) return launch_attend<TACO_F16, TACO_F16>(a, s);
+  if (c->dtype == TACO_BF16) return launch_attend<TACO_BF16, TACO_BF16>(a, s);
+  if (t->dtype == TACO_F16) return launch_attend<TACO_F16, TACO_E4M3>(a, s);
+  return launch_attend<TACO_BF16, TACO_E4M3>(a, s);
+}
+
+extern "C" int taco_kv_status(const taco_kv_cache* c, void* stream) {
+  if (!c || !c->flags) TACO_FAIL(TACO_EINVAL, "taco_kv_status: NULL argument");
+  DeviceScope on_device(c->device);
+  TACO_HIP(on_device.status);
+  hipStream_t s = (hipStream_t)stream;
+  uint32_t flags = 0;
+  const uint32_t zero = 0;
+  TACO_HIP(hipMemcpyAsync(&flags, c->flags, 4, hipMemcpyDeviceToHost, s));
+  TACO_HIP(hipStreamSynchronize(s));
+  if (!flags) return TACO_OK;
+  TACO_HIP(hipMemcpyAsync(c->flags, &zero, 4, hipMemcpyHostToDevice, s));
+  TACO_HIP(hipStreamSynchronize(s));
+  TACO_FAIL(TACO_ERANGE, "%s%s%s", flags & TACO_KV_BAD_PAGE ? "a table entry is no page of the cache" : "",
+            flags == (TACO_KV_BAD_PAGE | TACO_KV_BAD_PLACE) ? "; " : "", flags & TACO_KV_BAD_PLACE ? "a position or length lies outside the table" : "");
+}
