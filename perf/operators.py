@@ -210,7 +210,7 @@ def _prepare_w4(case, gen):
   s["x"] = _normal(gen, case["m"], k, dtype=case["dtype"])
   if own:
     from tacotron_amd.w4 import W4Matrix
-    s["handle"] = W4Matrix.from_codes(s["packed"], s["scales"], zeros=s["zeros"], bias=s["bias"], in_features=k)
+    s["handle"] = W4Matrix.from_codes(s["packed"], s["scales"], zeros=s["zeros"], bias=s["bias"], in_features=k, group=g)
   return s
 
 
