@@ -337,6 +337,38 @@ int64_t taco_kv_attend_workspace(const taco_kv_cache* cache, const taco_kv_atten
  * entry that is no page, or a position or length outside the table. */
 int taco_kv_status(const taco_kv_cache* cache, void* stream);
 
+/* A matrix [n_rows, n_cols] of 4-bit codes: W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), zero = 8
+ * where there are no zero points.  `packed` holds codes, scales and zero points in the order the kernel reads them, laid out
+ * once by taco_qmat_pack. */
+typedef struct taco_qmat {
+  const void* packed;         /* taco_qmat_bytes() bytes, 16-byte aligned */
+  const float* bias;          /* [n_rows] or NULL */
+  int32_t n_rows, n_cols;
+  int32_t group;              /* 32, 64 or 128 columns */
+  int32_t scale_dtype;        /* TACO_F32, TACO_F16 or TACO_BF16 */
+  int32_t has_zeros;
+  int32_t device;
+} taco_qmat;
+
+/* Size of `packed` for a matrix of these extents (its pointers are not looked at), or a negative code. */
+int64_t taco_qmat_bytes(const taco_qmat* m);
+
+/* Lays a matrix out: codes [n_rows, code_stride] bytes, two columns in each, the even one in the low half; scales [n_rows,
+ * scale_stride] of scale_dtype and zeros [n_rows, zero_stride] bytes (0 .. 15; NULL without has_zeros), one per group. */
+int taco_qmat_pack(const taco_qmat* m, const uint8_t* codes, int64_t code_stride, const void* scales, int64_t scale_stride,
+                   const uint8_t* zeros, int64_t zero_stride, void* packed, void* stream);
+
+/* Codes, scales (and zero points with has_zeros) of a matrix of weights [n_rows, weight_stride] of type `dtype`, as
+ * taco_qmat_pack takes them: the scale is max|w| / 7 of its group, or (max - min) / 15 with zero points (the interval holds
+ * 0), rounded to scale_dtype; a code is the nearest one to its weight.  Weights must be finite. */
+int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_stride, int32_t dtype, uint8_t* codes,
+                       int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
+
+/* y[v] = W x[v] + bias for n_vectors vectors x [n_vectors, x_stride] of type `dtype` (TACO_F32, TACO_F16, TACO_BF16), y
+ * [n_vectors, y_stride] of the same type; sums are fp32, rounded once.  W is read once for every 64 vectors. */
+int taco_qmat_multiply(const taco_qmat* m, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t n_vectors,
+                       int32_t dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@ EXPORTED_SYMBOLS = (
   "taco_encode", "taco_encode_status", "taco_decode", "taco_decode_resumable", "taco_postnet", "taco_postnet_noalloc", "taco_last_decode_timing",
   "taco_set_frame_clock", "taco_set_precision",
   "taco_kv_append", "taco_kv_attend", "taco_kv_attend_workspace", "taco_kv_status",
+  "taco_qmat_bytes", "taco_qmat_pack", "taco_qmat_quantize", "taco_qmat_multiply",
 )
 
 _lib: Optional[C.CDLL] = None
@@ -74,6 +75,12 @@ def lib() -> C.CDLL:
   L.taco_kv_attend_workspace.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAttendArgs)]
   L.taco_kv_attend_workspace.restype = C.c_int64
   L.taco_kv_status.argtypes = [C.POINTER(abi.TacoKvCache), vp]
+  qmat, i64 = C.POINTER(abi.TacoQmat), C.c_int64
+  L.taco_qmat_bytes.argtypes = [qmat]
+  L.taco_qmat_bytes.restype = i64
+  L.taco_qmat_pack.argtypes = [qmat, vp, i64, vp, i64, vp, i64, vp, vp]
+  L.taco_qmat_quantize.argtypes = [qmat, vp, i64, i32, vp, i64, vp, i64, vp, i64, vp]
+  L.taco_qmat_multiply.argtypes = [qmat, vp, i64, vp, i64, i32, i32, vp]
   _lib = L
   return L
 

@@ -85,6 +85,11 @@ class TacoKvAttendArgs(C.Structure):
   ] + [(n, C.c_int32) for n in ("window", "n_seqs", "table_width", "n_q_heads", "dtype")]
 
 
+class TacoQmat(C.Structure):
+  _fields_ = [("packed", C.c_void_p), ("bias", C.c_void_p)] + [
+    (n, C.c_int32) for n in ("n_rows", "n_cols", "group", "scale_dtype", "has_zeros", "device")]
+
+
 def build_dims(hp: HParams, n_symbols: int, n_stresses: Optional[int], n_speakers: Optional[int],
                n_tones: Optional[int], n_durations: Optional[int]) -> Tuple[TacoDims, ModelDims]:
   md = model_dims(hp, n_symbols, n_stresses, n_speakers, n_tones, n_durations)

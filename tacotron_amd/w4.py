@@ -1,0 +1,144 @@
+"""Matrices of 4-bit weights with group scales and their products with a few vectors, on the HIP library's ``taco_qmat_*``
+entry points (include/taco.h).  The reference has no counterpart: it computes with fp32 weights only."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Tuple
+
+import torch
+
+from tacotron_amd import _lib, abi
+
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _on_gpu(t: torch.Tensor, name: str) -> torch.device:
+  if t.device.type != "cuda":
+    raise RuntimeError(f"{name} must be on an AMD GPU (got device '{t.device}'); there is no CPU path")
+  return t.device
+
+
+def _check(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtypes, device: torch.device) -> None:
+  if tuple(t.shape) != shape or t.dtype not in dtypes or t.device != device:
+    raise ValueError(f"{name} must be {' or '.join(str(d) for d in dtypes)} {list(shape)} on {device}, got {t.dtype} "
+                     f"{tuple(t.shape)} on {t.device}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+  return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _pitch(t: torch.Tensor) -> int:
+  """Elements from row to row (a single row may have any stride)."""
+  return max(t.stride(0), t.shape[1])
+
+
+def quantize(weight: torch.Tensor, group: int = 128, symmetric: bool = True,
+             scale_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
+  """Codes, scales and zero points (None if ``symmetric``) of ``weight`` [out, in], which must be finite, as
+  ``W4Matrix.from_codes`` takes them: the scale of a group is max|w| / 7, or (max - min) / 15 with zero points, and a code the
+  nearest to its weight.  ``scale_dtype`` defaults to the weight's type."""
+  device = _on_gpu(weight, "weight")
+  if weight.dim() != 2 or weight.dtype not in _FLOATS or weight.numel() == 0:
+    raise ValueError(f"weight must be a float matrix, got {weight.dtype} {tuple(weight.shape)}")
+  scale_dtype = scale_dtype or weight.dtype
+  if group not in (32, 64, 128) or scale_dtype not in _FLOATS:
+    raise ValueError(f"groups are 32, 64 or 128 columns (got {group}), scales float32, float16 or bfloat16 (got {scale_dtype})")
+  n, k = weight.shape
+  groups = -(-k // group)
+  weight = _rows(weight)
+  codes = torch.empty(n, -(-k // 2), dtype=torch.uint8, device=device)
+  scales = torch.empty(n, groups, dtype=scale_dtype, device=device)
+  zeros = None if symmetric else torch.empty(n, groups, dtype=torch.uint8, device=device)
+  m = abi.TacoQmat(n_rows=n, n_cols=k, group=group, scale_dtype=abi.DTYPES[scale_dtype], has_zeros=not symmetric, device=device.index)
+  _lib.check(_lib.lib().taco_qmat_quantize(
+    C.byref(m), weight.data_ptr(), _pitch(weight), abi.DTYPES[weight.dtype], codes.data_ptr(), codes.shape[1], scales.data_ptr(),
+    groups, None if zeros is None else zeros.data_ptr(), groups, torch.cuda.current_stream(device).cuda_stream))
+  return codes, scales, zeros
+
+
+class W4Matrix:
+  """A matrix [out_features, in_features] of 4-bit codes: W[n, k] = scale[n, k // group] * (code[n, k] - zero[n, k // group]),
+  zero = 8 without zero points.  It owns a copy of them in the order the kernel reads, made once."""
+
+  def __init__(self, packed: torch.Tensor, bias: Optional[torch.Tensor], c: abi.TacoQmat):
+    self._packed, self._bias, self._c = packed, bias, c
+    self._ref = C.byref(c)
+    self.device, self.in_features, self.out_features, self.group = packed.device, c.n_cols, c.n_rows, c.group
+    self._lib = _lib.lib()
+
+  @classmethod
+  def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                 bias: Optional[torch.Tensor] = None, in_features: Optional[int] = None, group: Optional[int] = None) -> "W4Matrix":
+    """``codes`` uint8 [out, >= ceil(in / 2)], two columns in a byte, the even one in its low half; ``scales`` [out, groups]
+    float32, float16 or bfloat16; ``zeros`` uint8 [out, groups], 0 .. 15; ``bias`` [out].  ``in_features`` defaults to all the
+    codes there are; ``group`` (32, 64 or 128) to the one that the number of scales leaves."""
+    device = _on_gpu(codes, "codes")
+    if codes.dim() != 2 or codes.dtype != torch.uint8 or codes.numel() == 0:
+      raise ValueError(f"codes must be uint8 [out, in / 2], got {codes.dtype} {tuple(codes.shape)}")
+    n, k = codes.shape[0], 2 * codes.shape[1] if in_features is None else int(in_features)
+    if not 1 <= k <= 2 * codes.shape[1]:
+      raise ValueError(f"codes of {2 * codes.shape[1]} columns cannot have {k} in_features")
+    if scales.dim() != 2:
+      raise ValueError(f"scales must be [out, groups], got {tuple(scales.shape)}")
+    fits = [g for g in ((32, 64, 128) if group is None else (group,)) if g in (32, 64, 128) and -(-k // g) == scales.shape[1]]
+    if len(fits) != 1:
+      raise ValueError(f"{scales.shape[1]} scales a row for {k} columns fit groups of {fits or 'no allowed size'}"
+                       f"{'' if group is None else f' ({group} given)'}: groups are 32, 64 or 128 columns")
+    _check(scales, "scales", (n, scales.shape[1]), _FLOATS, device)
+    if zeros is not None:
+      _check(zeros, "zeros", tuple(scales.shape), (torch.uint8,), device)
+      zeros = _rows(zeros)
+    if bias is not None:
+      _check(bias, "bias", (n,), _FLOATS, device)
+      bias = bias.detach().to(torch.float32, copy=True).contiguous()
+    codes, scales = _rows(codes), _rows(scales)
+    m = abi.TacoQmat(n_rows=n, n_cols=k, group=fits[0], scale_dtype=abi.DTYPES[scales.dtype], has_zeros=zeros is not None,
+                     device=device.index)
+    L = _lib.lib()
+    size = L.taco_qmat_bytes(C.byref(m))
+    if size < 0:
+      _lib.check(int(size))
+    packed = torch.empty(size, dtype=torch.uint8, device=device)
+    _lib.check(L.taco_qmat_pack(
+      C.byref(m), codes.data_ptr(), _pitch(codes), scales.data_ptr(), _pitch(scales), None if zeros is None else zeros.data_ptr(),
+      0 if zeros is None else _pitch(zeros), packed.data_ptr(), torch.cuda.current_stream(device).cuda_stream))
+    m.packed, m.bias = packed.data_ptr(), None if bias is None else bias.data_ptr()
+    return cls(packed, bias, m)
+
+  @classmethod
+  def from_weights(cls, weight: torch.Tensor, group: int = 128, symmetric: bool = True, scale_dtype: Optional[torch.dtype] = None,
+                   bias: Optional[torch.Tensor] = None) -> "W4Matrix":
+    """The nearest 4-bit matrix to ``weight`` [out, in] (see ``quantize``)."""
+    codes, scales, zeros = quantize(weight, group, symmetric, scale_dtype)
+    return cls.from_codes(codes, scales, zeros=zeros, bias=bias, in_features=weight.shape[1], group=group)
+
+  @property
+  def nbytes(self) -> int:
+    """Bytes that a product reads of the matrix."""
+    return self._packed.numel()
+
+  def matvec(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x W^T + bias for vectors ``x`` [..., in_features] in float32, float16 or bfloat16; the result [..., out_features] has
+    x's type, its sums are fp32 and rounded once.  Meant for a few vectors (the matrix is read once for every 64)."""
+    shape, dtype = x.shape, x.dtype
+    if dtype not in _FLOATS or x.device != self.device or len(shape) < 1 or shape[-1] != self.in_features:
+      raise ValueError(f"x must be a float [..., {self.in_features}] tensor on {self.device}, got {dtype} {tuple(shape)} on {x.device}")
+    if len(shape) != 2:
+      x = x.reshape(-1, self.in_features)
+    x = _rows(x)
+    n = x.shape[0]
+    want = (*shape[:-1], self.out_features)
+    if out is None:
+      out = torch.empty(want, dtype=dtype, device=self.device)
+    elif out.shape != want or out.dtype != dtype or out.device != self.device or (out.dim() != 2 and not out.is_contiguous()) or \
+        (out.shape[-1] > 1 and out.stride(-1) != 1) or (n > 1 and out.dim() == 2 and out.stride(0) < self.out_features):
+      raise ValueError(f"out must be {dtype} {want} on {self.device}, its rows side by side, got {out.dtype} {tuple(out.shape)} "
+                       f"{out.stride()} on {out.device}")
+    if n:
+      if n > 1 and x.stride(0) < self.in_features:      # expanded or overlapping vectors
+        x = x.contiguous()
+      _lib.check(self._lib.taco_qmat_multiply(
+        self._ref, x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0) if len(shape) == 2 else self.out_features, n,
+        abi.DTYPES[dtype], torch.cuda.current_stream(self.device).cuda_stream))
+    return out

@@ -531,3 +531,190 @@ def test_two_streams_at_once():
   torch.cuda.synchronize()
   for i, (o, l) in enumerate(got):
     assert torch.equal(o, want[i % 2][0]) and torch.equal(l, want[i % 2][1])
+
+
+# ---- 4-bit matrices ---------------------------------------------------------------------------------------------------
+
+
+def make_codes(n, k, group, scale_dtype, zeros, g):
+  groups = -(-k // group)
+  codes = torch.randint(0, 16, (n, k), generator=g, device=DEV, dtype=torch.uint8)
+  flat = torch.nn.functional.pad(codes, (0, k % 2))
+  packed = flat[:, 0::2] | (flat[:, 1::2] << 4)
+  scales = (torch.rand(n, groups, generator=g, device=DEV) * 0.1 + 0.01).to(scale_dtype)
+  z = torch.randint(0, 16, (n, groups), generator=g, device=DEV, dtype=torch.uint8) if zeros else None
+  return codes, packed, scales, z
+
+
+def check_matvec(codes, scales, zeros, group, bias, x, got):
+  """A group's sum of c x in fp32 is off by at most (group + 8) U of the sum of |terms|; taking the offset off and
+  scaling adds a few U more, the groups' and the eight waves' sums (groups + 16) U.  The terms are (c - z) x for fp32, c x and
+  z sum x for float16, (128 + c) x and (128 + z) sum x for bfloat16; then the bias and one rounding."""
+  n, k = codes.shape
+  s = scales.double().repeat_interleave(group, 1)[:, :k]
+  z = torch.full_like(s, 8.0) if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
+  c, x64 = codes.double(), x.double()
+  want = x64 @ ((c - z) * s).t()
+  size = {F32: (c - z).abs(), F16: c + z, BF16: 256 + c + z}[x.dtype] * s
+  if bias is not None:
+    want = want + bias.double()
+  slack = (group + 8 + scales.shape[1] + 16 + 8) * U * (x64.abs() @ size.t()) + 2 * U * want.abs()
+  tol = slack + half_step(x.dtype) * (want.abs() + slack) + (2.0 ** -25 if x.dtype == F16 else 0)
+  excess = (got.double() - want).abs() - tol
+  assert excess.max().item() <= 0, (excess.max().item(), want.flatten()[excess.argmax()].item())
+
+
+MATVECS = [
+  # x, scales, vectors, out, in, group, zeros, bias
+  (F32, F32, 1, 1, 1, 32, False, False),
+  (F32, F32, 1, 80, 1558, 32, False, True),
+  (F32, F16, 16, 17, 129, 128, True, False),
+  (F32, BF16, 17, 100, 333, 64, True, True),
+  (F32, F32, 65, 33, 127, 32, True, False),
+  (F16, F16, 1, 4096, 1024, 128, False, False),
+  (F16, F32, 3, 15, 31, 32, True, True),
+  (F16, F16, 33, 16, 128, 64, True, False),
+  (F16, BF16, 5, 1000, 97, 128, False, True),
+  (BF16, BF16, 1, 31, 4099, 128, True, False),
+  (BF16, F32, 2, 48, 2048, 32, True, True),
+  (BF16, F16, 16, 130, 1000, 64, False, False),
+  (BF16, BF16, 130, 50, 65, 32, False, True),
+  (BF16, BF16, 1, 3, 20000, 128, True, False),
+]
+
+
+@pytest.mark.parametrize("dtype,scale_dtype,vectors,n,k,group,zeros,with_bias", MATVECS)
+def test_matvec(dtype, scale_dtype, vectors, n, k, group, zeros, with_bias):
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(n + k)
+  codes, packed, scales, z = make_codes(n, k, group, scale_dtype, zeros, g)
+  bias = torch.randn(n, generator=g, device=DEV).to(dtype) if with_bias else None
+  W = W4Matrix.from_codes(packed, scales, zeros=z, bias=bias, in_features=k, group=group)
+  assert (W.out_features, W.in_features, W.group) == (n, k, group)
+  x = torch.randn(vectors, k, generator=g, device=DEV).to(dtype)
+  got = W.matvec(x)
+  check_matvec(codes, scales, z, group, bias, x, got)
+  assert torch.equal(W.matvec(x), got)
+  # every vector alone, rows of a wider tensor at odd addresses, and into a given output
+  wide = torch.full((vectors, k + 3), float("nan"), dtype=dtype, device=DEV)
+  wide[:, 1:k + 1] = x
+  into = torch.full((vectors, n + 5), 7.0, dtype=dtype, device=DEV)
+  W.matvec(wide[:, 1:k + 1], out=into[:, 2:n + 2])
+  assert torch.equal(into[:, 2:n + 2], got) and bool((into[:, :2] == 7).all()) and bool((into[:, n + 2:] == 7).all())
+  check_matvec(codes, scales, z, group, bias, x[-1:], W.matvec(x[-1])[None])
+  assert W.matvec(x.reshape(1, vectors, k)).shape == (1, vectors, n)
+  assert W.matvec(x[:0]).shape == (0, n)
+
+
+def test_matvec_extreme_codes_and_values():
+  """All codes at either end, inputs from the smallest subnormals to the largest finite ones."""
+  from tacotron_amd.w4 import W4Matrix
+  for dtype, values_ in ((F16, [6e-8, 6e-5, 1.0, 60000.0]), (BF16, [1e-38, 1e-30, 1.0, 1e30]), (F32, [1e-38, 1e-30, 1.0, 1e30])):
+    for code, zero in ((0, 0), (0, 15), (15, 0), (15, 15), (7, 8)):
+      z = torch.full((16, 1), zero, dtype=torch.uint8, device=DEV)
+      scales = torch.full((16, 1), 1e-3, device=DEV)
+      W = W4Matrix.from_codes(torch.full((16, 32), code * 17, dtype=torch.uint8, device=DEV), scales, zeros=z, group=64)
+      for v in values_:
+        x = torch.full((1, 64), v, dtype=dtype, device=DEV)
+        x[0, ::3] *= -1
+        got = W.matvec(x)
+        size = {F32: abs(code - zero), F16: code + zero, BF16: 256 + code + zero}[dtype] * 1e-3 * x.double().abs().sum().item()
+        want = (code - zero) * scales[0].double() * x.double().sum()
+        tol = 110 * U * size + half_step(dtype) * want.abs() + {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
+        assert ((got.double() - want).abs() <= tol).all(), (dtype, code, zero, v)
+
+
+@pytest.mark.parametrize("dtype,scale_dtype,n,k,group,symmetric", [
+  (F32, None, 5, 97, 32, True), (F32, F16, 3, 128, 64, False), (BF16, None, 17, 1000, 128, True), (F16, F32, 1, 1, 32, False),
+  (BF16, F32, 33, 65, 64, False)])
+def test_quantize(dtype, scale_dtype, n, k, group, symmetric):
+  from tacotron_amd import w4
+  g = gen(k)
+  w = torch.randn(n, k + 2, generator=g, device=DEV).to(dtype)[:, :k]
+  w[0, :min(k, group)] = 0                              # a group of zeros
+  codes, scales, zeros = w4.quantize(w, group, symmetric, scale_dtype)
+  assert scales.dtype == (scale_dtype or dtype) and (zeros is None) == symmetric
+  groups = -(-k // group)
+  full = torch.nn.functional.pad(w.float().cpu(), (0, groups * group - k)).view(n, groups, group)
+  lo, hi = full.amin(-1).clamp(max=0), full.amax(-1).clamp(min=0)
+  s = ((torch.maximum(hi, -lo) / 7) if symmetric else (hi - lo) / 15).to(scales.dtype)
+  assert torch.equal(scales.cpu(), s)
+  s = s.float()[..., None]
+  z = torch.full_like(s, 8.0) if symmetric else torch.where(s > 0, (-lo[..., None] / s).round().clamp(0, 15), 0.0)
+  q = torch.where(s > 0, ((full / s).round() + z).clamp(0, 15), z).to(torch.uint8).flatten(1)[:, :k]
+  unpacked = torch.stack([codes & 15, codes >> 4], -1).flatten(1)[:, :k].cpu()
+  assert torch.equal(unpacked, q)
+  if zeros is not None:
+    assert torch.equal(zeros.cpu().float(), z[..., 0])
+  W = w4.W4Matrix.from_weights(w, group, symmetric, scale_dtype)
+  x = torch.randn(2, k, generator=g, device=DEV)
+  check_matvec(unpacked.to(DEV), scales, zeros, group, None, x, W.matvec(x))
+
+
+def test_matvec_refusals():
+  from tacotron_amd.w4 import W4Matrix, quantize
+  codes, packed, scales, z = make_codes(8, 64, 32, F32, True, gen(1))
+  W = W4Matrix.from_codes(packed, scales, zeros=z)
+  x = torch.zeros(2, 64, device=DEV)
+  for call in (
+    lambda: W4Matrix.from_codes(packed, scales, in_features=65), lambda: W4Matrix.from_codes(packed, scales, in_features=0),
+    lambda: W4Matrix.from_codes(packed, scales[:, :1], in_features=30), lambda: W4Matrix.from_codes(packed, scales, group=16),
+    lambda: W4Matrix.from_codes(packed, scales[:4]), lambda: W4Matrix.from_codes(packed.int(), scales), lambda: W4Matrix.from_codes(packed, scales.double()),
+    lambda: W4Matrix.from_codes(packed, scales, zeros=z[:, :1]), lambda: W4Matrix.from_codes(packed, scales, zeros=z.int()),
+    lambda: W4Matrix.from_codes(packed, scales, bias=torch.zeros(7, device=DEV)), lambda: W4Matrix.from_codes(packed.cpu(), scales.cpu()),
+    lambda: W.matvec(x[:, :63]), lambda: W.matvec(x.double()), lambda: W.matvec(x.cpu()), lambda: W.matvec(x, out=torch.zeros(2, 9, device=DEV)),
+    lambda: W.matvec(x, out=torch.zeros(8, 2, device=DEV).t()), lambda: W.matvec(x, out=torch.zeros(1, 8, device=DEV).expand(2, 8)),
+    lambda: quantize(torch.zeros(3, 0, device=DEV)), lambda: quantize(torch.zeros(3, 8, device=DEV), group=48), lambda: quantize(torch.zeros(3, 8)),
+  ):
+    with pytest.raises((ValueError, RuntimeError)):
+      call()
+
+
+# ---- a run of them together ---------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (F16, E4M3)])
+def test_layers_of_a_decoder_step(dtype, held):
+  """Prompts of several utterances, then single frames, through two layers: projection, append, attend, projection.  Every
+  operator is checked against 64 bits on what the one before it gave."""
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(21)
+  width, hq, hkv, d, page, layers = 256, 4, 2, 64, 16, 2
+  qkv = hq + 2 * hkv
+  weights = []
+  for _ in range(layers):
+    for n, k in ((qkv * d, width), (width, hq * d)):
+      codes, packed, scales, z = make_codes(n, k, 64, F32 if dtype == F32 else dtype, True, g)
+      weights.append((codes, scales, z, W4Matrix.from_codes(packed, scales, zeros=z, group=64)))
+  caches = [make_cache(24, page, hkv, d, held, g) for _ in range(layers)]
+  table = make_table([5, 4, 6], 24, 6, 3)
+  inv_freq = 10000.0 ** (-torch.arange(d // 2, dtype=torch.float64, device=DEV) / (d // 2))
+  past = [0, 0, 0]
+  for new in ([15, 33, 60], [1, 1, 1], [1, 1, 1], [2, 0, 1], [1, 1, 1]):
+    x = (torch.randn(sum(new), width, generator=g, device=DEV) * 0.1).to(dtype)
+    offsets = torch.tensor([0] + new, device=DEV).cumsum(0).to(torch.int32)
+    single = all(n == 1 for n in new)
+    past_dev = torch.tensor(past, dtype=torch.int32, device=DEV)
+    lens = [p + n for p, n in zip(past, new)]
+    for layer in range(layers):
+      codes, scales, z, W = weights[2 * layer]
+      h = W.matvec(x)
+      check_matvec(codes, scales, z, 64, None, x, h)
+      h = (h / h.float().abs().mean()).to(dtype).view(-1, qkv, d)
+      q, k, v = h[:, :hq], h[:, hq:hq + hkv], h[:, hq + hkv:]
+      cache = caches[layer]
+      before = cache.k.clone(), cache.v.clone()
+      turned = cache.append(k, v, table, past_dev, q=q, offsets=None if single else offsets, inv_freq=inv_freq)
+      check_append(cache, k, v, q, table, past, new, inv_freq, False, turned, before)
+      # the last token of every utterance that has one attends
+      rows = [b for b, n in enumerate(new) if n]
+      last = torch.tensor([int(offsets[b + 1]) - 1 for b in rows], device=DEV)
+      got = cache.attend(turned[last], table[rows], torch.tensor([lens[b] for b in rows], dtype=torch.int32, device=DEV), return_lse=True)
+      check_attend(cache, turned[last], table[rows], [lens[b] for b in rows], d ** -0.5, 0, got)
+      cache.check()
+      codes, scales, z, W = weights[2 * layer + 1]
+      y = W.matvec(got[0].flatten(1))
+      check_matvec(codes, scales, z, 64, None, got[0].flatten(1), y)
+      x = x.clone()
+      x[last] += (y / y.float().abs().mean() * 0.1).to(dtype)
+    past = lens

@@ -121,16 +121,73 @@ def test_nothing_to_do_and_null_arguments():
 
 
 def test_struct_layouts_match_the_header(tmp_path):
-  names = ["taco_kv_cache", "taco_kv_append_args", "taco_kv_attend_args"]
+  names = ["taco_kv_cache", "taco_kv_append_args", "taco_kv_attend_args", "taco_qmat"]
   src = tmp_path / "s.c"
   src.write_text('#include <stdio.h>\n#include "taco.h"\nint main(void) { printf("' + "%zu " * len(names) + '\\n", ' +
                  ", ".join(f"sizeof({n})" for n in names) + "); return 0; }\n")
   subprocess.check_call(["cc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "s")])
   sizes = [int(v) for v in subprocess.check_output([str(tmp_path / "s")]).split()]
-  assert sizes == [C.sizeof(t) for t in (abi.TacoKvCache, abi.TacoKvAppendArgs, abi.TacoKvAttendArgs)]
+  assert sizes == [C.sizeof(t) for t in (abi.TacoKvCache, abi.TacoKvAppendArgs, abi.TacoKvAttendArgs, abi.TacoQmat)]
 
 
 def test_the_cache_has_no_cpu_path():
   from tacotron_amd.paged import PagedCache
   with pytest.raises(RuntimeError):
     PagedCache(2, 16, 1, 64, device="cpu")
+
+
+def _qmat(**change):
+  return abi.TacoQmat(**{**dict(packed=4096, n_rows=32, n_cols=100, group=64, scale_dtype=abi.TACO_F16), **change})
+
+
+def test_size_of_a_packed_matrix():
+  """Blocks of 16 x 128 codes (1 KiB), then 16 scales, then 16 zero points per block row and group."""
+  L = _lib.lib()
+  for n, k, group, dtype, zeros, want in (
+    (32, 100, 64, abi.TACO_F16, 0, 2 * 1024 + 2 * 2 * 32), (32, 100, 64, abi.TACO_F16, 1, 2 * 1024 + 2 * 2 * 32 + 2 * 2 * 16),
+    (1, 1, 32, abi.TACO_F32, 0, 1024 + 4 * 64), (17, 129, 128, abi.TACO_BF16, 1, 4 * 1024 + 4 * 32 + 4 * 16),
+    (28672, 8192, 128, abi.TACO_BF16, 0, 28672 * 4096 + 28672 * 64 * 2),
+    (1 << 20, 1 << 20, 128, abi.TACO_F32, 0, (1 << 39) + (1 << 35))):
+    assert L.taco_qmat_bytes(C.byref(_qmat(n_rows=n, n_cols=k, group=group, scale_dtype=dtype, has_zeros=zeros))) == want
+
+
+@pytest.mark.parametrize("change,word", [
+  (dict(n_rows=0), "rows"), (dict(n_cols=0), "columns"), (dict(n_rows=1 << 29), "rows"), (dict(group=16), "group"), (dict(group=0), "group"),
+  (dict(scale_dtype=3), "scale_dtype"), (dict(scale_dtype=-1), "scale_dtype")])
+def test_bad_matrices_are_refused(change, word):
+  L, m = _lib.lib(), _qmat(**change)
+  calls = (lambda: L.taco_qmat_pack(C.byref(m), 64, 50, 64, 2, None, 0, 64, None),
+           lambda: L.taco_qmat_quantize(C.byref(m), 64, 100, 0, 64, 50, 64, 2, None, 0, None),
+           lambda: L.taco_qmat_multiply(C.byref(m), 64, 100, 64, 32, 1, 0, None))
+  for call in calls:
+    with pytest.raises(_lib.TacoError) as e:
+      _lib.check(call())
+    assert e.value.code == abi.TACO_EINVAL and word in str(e.value)
+  assert L.taco_qmat_bytes(C.byref(m)) == abi.TACO_EINVAL
+
+
+def test_bad_matrix_calls_are_refused():
+  L, m, mz = _lib.lib(), C.byref(_qmat()), C.byref(_qmat(has_zeros=1))
+  for rc in (
+    L.taco_qmat_bytes(None), L.taco_qmat_pack(None, 64, 50, 64, 2, None, 0, 64, None), L.taco_qmat_pack(m, None, 50, 64, 2, None, 0, 64, None),
+    L.taco_qmat_pack(m, 64, 49, 64, 2, None, 0, 64, None), L.taco_qmat_pack(m, 64, 50, 64, 1, None, 0, 64, None),
+    L.taco_qmat_pack(m, 64, 50, 64, 2, 64, 2, 64, None), L.taco_qmat_pack(mz, 64, 50, 64, 2, None, 0, 64, None),
+    L.taco_qmat_pack(mz, 64, 50, 64, 2, 64, 1, 64, None), L.taco_qmat_pack(m, 64, 50, 64, 2, None, 0, 72, None),
+    L.taco_qmat_quantize(m, 64, 99, 0, 64, 50, 64, 2, None, 0, None), L.taco_qmat_quantize(m, 64, 100, 3, 64, 50, 64, 2, None, 0, None),
+    L.taco_qmat_quantize(m, None, 100, 0, 64, 50, 64, 2, None, 0, None), L.taco_qmat_quantize(mz, 64, 100, 0, 64, 50, 64, 2, None, 0, None),
+    L.taco_qmat_multiply(m, 64, 100, 64, 32, -1, 0, None), L.taco_qmat_multiply(m, 64, 100, 64, 32, 1, 3, None),
+    L.taco_qmat_multiply(m, None, 100, 64, 32, 1, 0, None), L.taco_qmat_multiply(m, 64, 100, None, 32, 1, 0, None),
+    L.taco_qmat_multiply(m, 66, 100, 64, 32, 1, 0, None), L.taco_qmat_multiply(m, 64, 99, 64, 32, 2, 0, None),
+    L.taco_qmat_multiply(m, 64, 100, 64, 31, 2, 0, None), L.taco_qmat_multiply(C.byref(_qmat(packed=None)), 64, 100, 64, 32, 1, 0, None),
+    L.taco_qmat_multiply(C.byref(_qmat(packed=4104)), 64, 100, 64, 32, 1, 0, None)):
+    assert rc == abi.TACO_EINVAL
+  assert L.taco_qmat_multiply(m, 64, 100, 64, 32, 0, 0, None) == 0
+
+
+def test_matrices_have_no_cpu_path():
+  import torch
+  from tacotron_amd import w4
+  with pytest.raises(RuntimeError):
+    w4.quantize(torch.zeros(4, 64))
+  with pytest.raises(RuntimeError):
+    w4.W4Matrix.from_codes(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2))
