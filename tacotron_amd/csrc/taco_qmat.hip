@@ -172,9 +172,11 @@ __device__ __forceinline__ taco_f4 load_scales(const char* p, int dtype) {
 
 // One workgroup per 16 rows of W and 16 * MT vectors; its NW waves take the row block's 128-column blocks in turn and
 // are summed through LDS in their order.
-//   16-bit x: a pair of nibbles becomes a pair of operands without a conversion.  bfloat16: 0x4300 | code is 128 + code;
-//     float16: the code alone is the subnormal code * 2^-24, which the matrix cores take as it is.  The offset 128 and the
-//     zero point come off per group: sum (c - z) x = sum c' x - (offset + z) sum x, sum x from a product with ones.
+//   16-bit x: a pair of nibbles becomes a pair of operands without a conversion.
+//     bfloat16: 0x4300 | code is 128 + code.  That offset and the zero point come off per group: sum (c - z) x = sum (128 + c) x -
+//     (128 + z) sum x, sum x from a product with ones (v_mfma_f32_16x16x32 is not what bounds this).
+//     float16: 0x6400 | code is 1024 + code; one packed subtraction leaves c - z, exactly.  (The code alone, the subnormal
+//     c * 2^-24, would save it, but the matrix cores lose bits of sums of such products: 2^-15 of the result measured.)
 //   fp32 x: codes are converted (a byte at a time) and lose their zero point there, exactly; v_mfma_f32_16x16x4_f32.
 template <int T, int MT, int NW>
 __global__ __launch_bounds__(64 * NW) void taco_qmat_multiply_kernel(const MultiplyParams a) {
@@ -221,28 +223,36 @@ __global__ __launch_bounds__(64 * NW) void taco_qmat_multiply_kernel(const Multi
           for (int m = 0; m < MT; ++m) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(c, x[m].v[e], acc[m], 0, 0, 0);
         }
       } else {
-        constexpr uint32_t over = T == TACO_BF16 ? 0x43004300u : 0u, one = T == TACO_BF16 ? 0x3f803f80u : 0x00010001u;
-        const taco_u4 c = {(w[j] & 0x000f000fu) | over, ((w[j] >> 4) & 0x000f000fu) | over, ((w[j] >> 8) & 0x000f000fu) | over,
-                           ((w[j] >> 12) & 0x000f000fu) | over};
+        constexpr uint32_t over = T == TACO_BF16 ? 0x43004300u : 0x64006400u;
+        taco_u4 c = {(w[j] & 0x000f000fu) | over, ((w[j] >> 4) & 0x000f000fu) | over, ((w[j] >> 8) & 0x000f000fu) | over,
+                     ((w[j] >> 12) & 0x000f000fu) | over};
+        if constexpr (T == TACO_F16) {
+          _Float16 z = (_Float16)1032.0f;
+          if (zeros) z = (_Float16)(1024.0f + (float)(uint8_t)zeros[group * 16 + r]);
+          const taco_h2 zz = {z, z};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t pair = c[e];     // a copy: __builtin_bit_cast of a vector's element takes its first one here
+            c[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(taco_h2, pair) - zz);
+          }
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           acc[m] = taco_mfma32<T>(c, x[m].v, acc[m]);
-          sum[m] = taco_mfma32<T>(taco_u4{one, one, one, one}, x[m].v, sum[m]);
+          if constexpr (T == TACO_BF16) sum[m] = taco_mfma32<T>(taco_u4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u}, x[m].v, sum[m]);
         }
       }
       if ((j & last) == last) {
-        taco_f4 s = load_scales(scales + (int64_t)group * 16 * ssize, a.scale_dtype);
-        if constexpr (T == TACO_F32) {
+        const taco_f4 s = load_scales(scales + (int64_t)group * 16 * ssize, a.scale_dtype);
+        if constexpr (T != TACO_BF16) {
 #pragma unroll
           for (int m = 0; m < MT; ++m) y[m] += s * acc[m];
         } else {
-          taco_f4 off = taco_f4{8, 8, 8, 8};
+          taco_f4 off = taco_f4{136, 136, 136, 136};
           if (zeros) {
             const uint32_t z = *(const uint32_t*)(zeros + group * 16 + g * 4);
-            off = taco_f4{(float)(z & 255), (float)((z >> 8) & 255), (float)((z >> 16) & 255), (float)(z >> 24)};
+            off = taco_f4{(float)(z & 255), (float)((z >> 8) & 255), (float)((z >> 16) & 255), (float)(z >> 24)} + 128.0f;
           }
-          if (T == TACO_BF16) off += 128.0f;
-          else s *= 16777216.0f;
 #pragma unroll
           for (int m = 0; m < MT; ++m) y[m] += s * (acc[m] - off * sum[m]);
         }

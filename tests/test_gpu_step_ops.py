@@ -548,14 +548,14 @@ def make_codes(n, k, group, scale_dtype, zeros, g):
 
 def check_matvec(codes, scales, zeros, group, bias, x, got):
   """A group's sum of c x in fp32 is off by at most (group + 8) U of the sum of |terms|; taking the offset off and
-  scaling adds a few U more, the groups' and the eight waves' sums (groups + 16) U.  The terms are (c - z) x for fp32, c x and
-  z sum x for float16, (128 + c) x and (128 + z) sum x for bfloat16; then the bias and one rounding."""
+  scaling adds a few U more, the groups' and the waves' sums (groups + 16) U.  The terms are (c - z) x for fp32 and float16,
+  (128 + c) x and (128 + z) sum x for bfloat16; then the bias and one rounding."""
   n, k = codes.shape
   s = scales.double().repeat_interleave(group, 1)[:, :k]
   z = torch.full_like(s, 8.0) if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
   c, x64 = codes.double(), x.double()
   want = x64 @ ((c - z) * s).t()
-  size = {F32: (c - z).abs(), F16: c + z, BF16: 256 + c + z}[x.dtype] * s
+  size = (256 + c + z if x.dtype == BF16 else (c - z).abs()) * s
   if bias is not None:
     want = want + bias.double()
   slack = (group + 8 + scales.shape[1] + 16 + 8) * U * (x64.abs() @ size.t()) + 2 * U * want.abs()
@@ -618,7 +618,7 @@ def test_matvec_extreme_codes_and_values():
         x = torch.full((1, 64), v, dtype=dtype, device=DEV)
         x[0, ::3] *= -1
         got = W.matvec(x)
-        size = {F32: abs(code - zero), F16: code + zero, BF16: 256 + code + zero}[dtype] * 1e-3 * x.double().abs().sum().item()
+        size = (256 + code + zero if dtype == BF16 else abs(code - zero)) * 1e-3 * x.double().abs().sum().item()
         want = (code - zero) * scales[0].double() * x.double().sum()
         tol = 110 * U * size + half_step(dtype) * want.abs() + {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
         assert ((got.double() - want).abs() <= tol).all(), (dtype, code, zero, v)
