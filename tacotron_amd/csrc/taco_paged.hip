@@ -4,6 +4,7 @@
 #include "taco_step.h"
 
 #include <atomic>
+#include <type_traits>
 
 namespace {
 
@@ -147,8 +148,10 @@ struct AttendParams {
   uint32_t* flags;
   int64_t table_stride;
   taco_divisor page16;                                    // 16-token blocks of a page
+  float* partial;                                    // [2 * workgroups][rows][2 + DP], see Shares
   float scale_log2;                                  // scale * log2(e)
   int32_t n_seqs, table_width, n_pages, n_heads, n_q_heads, group, q_tiles, head_dim, window;
+  int32_t least;                                     // tiles of a workgroup's share at least
 };
 
 constexpr int AT_WAVES = 4;
@@ -367,65 +370,186 @@ struct Attend {
   }
 };
 
-// One workgroup per (utterance, cache head, 16 of its query heads): its waves take the tiles in turn and are joined
-// through LDS.
+// ---- who does what ----
+// All tiles of a call stand in one line: utterance by utterance, within it row by row (a row: one cache head and up to 16 of
+// its query heads), within a row from the first seen tile to the last.  The line is cut into equal shares, one per
+// workgroup of a grid that fills the GPU once, whatever the lengths are: a long utterance alone is split over its length,
+// a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
+// by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
+// kernel joins in the order of the workgroups.
+struct Span {
+  int low, len;        // seen tokens [low, len)
+  uint32_t tiles;      // of one row; an utterance that sees nothing has one, so that somebody writes its zeros
+};
+__device__ __forceinline__ Span span_of(const AttendParams& a, int b, int tt, bool flag) {
+  Span s;
+  s.len = a.lens[b];
+  const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
+  if (s.len < 0 || s.len > room) {
+    if (flag) atomicOr(a.flags, TACO_KV_BAD_PLACE);
+    s.len = s.len < 0 ? 0 : (int)room;
+  }
+  s.low = a.window > 0 ? max(0, s.len - a.window) : 0;
+  s.tiles = s.len > s.low ? (uint32_t)((s.len + tt - 1) / tt - s.low / tt) : 1;
+  return s;
+}
+// Inclusive sum over the lanes of a wave.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t u = __shfl_up(v, d, 64);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+// Tiles of one row of every utterance, summed over the utterances (every wave for itself, 64 utterances at a time).
+__device__ __forceinline__ uint32_t all_tiles(const AttendParams& a, int tt) {
+  uint32_t sum = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) {
+    const int b = i + (threadIdx.x & 63);
+    const uint32_t t = b < a.n_seqs ? span_of(a, b, tt, blockIdx.x == 0 && threadIdx.x < 64).tiles : 0;
+    sum += __builtin_amdgcn_readlane(wave_scan(t), 63);
+  }
+  return sum;
+}
+// The utterance that tile `at` (counted with one row per utterance) belongs to, and the tiles before it.
+__device__ __forceinline__ int find_utterance(const AttendParams& a, int tt, uint32_t at, uint32_t& before) {
+  uint32_t sum = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) {
+    const int b = i + (threadIdx.x & 63);
+    const uint32_t t = b < a.n_seqs ? span_of(a, b, tt, false).tiles : 0, scan = wave_scan(t), all = __builtin_amdgcn_readlane(scan, 63);
+    if (at - sum < all) {
+      const int n = __popcll(__ballot(sum + scan <= at));       // utterances of this 64 that end at or before `at`
+      before = sum + (n ? __builtin_amdgcn_readlane(scan, n - 1) : 0);
+      return i + n;
+    }
+    sum += all;
+  }
+  before = sum;
+  return a.n_seqs;
+}
+__device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all, uint32_t workgroups) {
+  const uint64_t share = (all + workgroups - 1) / workgroups;
+  return share < (uint64_t)a.least ? (uint64_t)a.least : share;
+}
+
+template <int T>
+__device__ __forceinline__ void store_out(char* row, int d, float o) {
+  if constexpr (T == TACO_F32) ((float*)row)[d] = o;
+  else if constexpr (T == TACO_BF16) ((__bf16*)row)[d] = (__bf16)o;
+  else ((_Float16*)row)[d] = (_Float16)o;
+}
+// Element d of query r of a row from `n` partial results part(i): final, or partial again where `leave` is given.
+template <int T, int C, int DP, typename Part>
+__device__ __forceinline__ void join(const AttendParams& a, int b, int h, int qt, int r, int d, int n, Part part, float* leave) {
+  float m = NEG_INF;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, part(i)[0]);
+  float sum = 0.0f, o = 0.0f;
+  for (int i = 0; i < n; ++i) {
+    const float* p = part(i);
+    const float f = p[0] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
+    sum += f * p[1];
+    o += f * p[2 + d];
+  }
+  if (leave) {
+    if (d == 0) { leave[0] = m; leave[1] = sum; }
+    leave[2 + d] = o;
+    return;
+  }
+  if (d >= a.head_dim) return;
+  const int head = h * a.group + qt * 16 + r;
+  o = sum == 0.0f ? 0.0f : o / sum * (C == TACO_E4M3 ? a.v_scale[h] : 1.0f);
+  store_out<T>(a.out + (int64_t)b * a.o_st[0] + (int64_t)head * a.o_st[1], d, o);
+  if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+}
+
 template <int T, int C, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const AttendParams a) {
   using A = Attend<T, C, DP>;
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
-  const int qt = blockIdx.x % a.q_tiles, bh = blockIdx.x / a.q_tiles, h = bh % a.n_heads, b = bh / a.n_heads;
-  const int rows = min(a.group - qt * 16, 16);
-  int len = a.lens[b];
-  const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
-  if (len < 0 || len > room) {
-    if (threadIdx.x == 0) atomicOr(a.flags, TACO_KV_BAD_PLACE);
-    len = len < 0 ? 0 : (int)room;
-  }
-  const int low = a.window > 0 ? max(0, len - a.window) : 0;
-  taco_u4 q[A::NQ];
-  A::load_q(a, b, h, qt, q);
-  float factor = a.scale_log2;
-  if (C == TACO_E4M3) factor *= a.k_scale[h];
-  typename A::St st;
-#pragma unroll
-  for (int blk = 0; blk < A::NB; ++blk)
-#pragma unroll
-    for (int e = 0; e < A::VE; ++e) st.o[blk][e] = taco_f4{0, 0, 0, 0};
-  for (int t0 = low / A::TT * A::TT + wave * A::TT; t0 < len; t0 += AT_WAVES * A::TT) A::tile(a, b, h, t0, low, len, factor, q, st);
-  // join the waves: [wave][query][m, l, DP outputs]
-  const float l = taco_sum_rows(st.l);
-  float* mine = lds + (wave * rows + col) * (DP + 2);
-  if (col < rows) {
-    if (g == 0) { mine[0] = st.m; mine[1] = l; }
+  const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
+  const uint64_t all = (uint64_t)all_tiles(a, A::TT) * rows_per, share = share_of(a, all, gridDim.x);
+  uint64_t at = share * blockIdx.x;
+  const uint64_t end = at + share < all ? at + share : all;
+  if (at >= end) return;
+  uint32_t before;
+  int b = find_utterance(a, A::TT, (uint32_t)(at / rows_per), before);
+  const int held = a.group < 16 ? a.group : 16;            // queries of a row in LDS and in the partial results
+  bool first = true;
+  uint64_t in = at - (uint64_t)before * rows_per;          // tile within the utterance
+  while (at < end) {
+    const Span sp = span_of(a, b, A::TT, false);
+    const uint32_t row = (uint32_t)(in / sp.tiles), tile0 = (uint32_t)(in - (uint64_t)row * sp.tiles);
+    const uint32_t n = (uint32_t)(end - at < sp.tiles - tile0 ? end - at : sp.tiles - tile0);
+    const int qt = row % a.q_tiles, h = row / a.q_tiles;
+    taco_u4 q[A::NQ];
+    A::load_q(a, b, h, qt, q);
+    float factor = a.scale_log2;
+    if (C == TACO_E4M3) factor *= a.k_scale[h];
+    typename A::St st;
 #pragma unroll
     for (int blk = 0; blk < A::NB; ++blk)
 #pragma unroll
-      for (int e = 0; e < A::VE; ++e)
+      for (int e = 0; e < A::VE; ++e) st.o[blk][e] = taco_f4{0, 0, 0, 0};
+    const int base = (sp.low / A::TT + (int)tile0) * A::TT;
+    if (sp.len > sp.low)
+      for (uint32_t t = wave; t < n; t += AT_WAVES) A::tile(a, b, h, base + (int)t * A::TT, sp.low, sp.len, factor, q, st);
+    // join the waves: [wave][query][m, l, DP outputs]
+    if (!first) __syncthreads();
+    first = false;
+    const float l = taco_sum_rows(st.l);
+    if (col < held) {
+      float* mine = lds + (wave * held + col) * (DP + 2);
+      if (g == 0) { mine[0] = st.m; mine[1] = l; }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mine[2 + blk * 16 * A::VE + (4 * g + i) * A::VE + e] = st.o[blk][e][i];
-  }
-  __syncthreads();
-  const float v_scale = C == TACO_E4M3 ? a.v_scale[h] : 1.0f;
-  for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
-    const int r = i / DP, d = i % DP;
-    if (d >= a.head_dim) continue;
-    float m = NEG_INF;
-    for (int w = 0; w < AT_WAVES; ++w) m = fmaxf(m, lds[(w * rows + r) * (DP + 2)]);
-    float sum = 0.0f, o = 0.0f;
-    for (int w = 0; w < AT_WAVES; ++w) {
-      const float* p = lds + (w * rows + r) * (DP + 2);
-      const float f = p[0] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
-      sum += f * p[1];
-      o += f * p[2 + d];
+      for (int blk = 0; blk < A::NB; ++blk)
+#pragma unroll
+        for (int e = 0; e < A::VE; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mine[2 + blk * 16 * A::VE + (4 * g + i) * A::VE + e] = st.o[blk][e][i];
     }
-    const int head = h * a.group + qt * 16 + r;
-    o = sum == 0.0f ? 0.0f : o / sum * v_scale;
-    char* out = a.out + (int64_t)b * a.o_st[0] + (int64_t)head * a.o_st[1];
-    if constexpr (T == TACO_F32) ((float*)out)[d] = o;
-    else if constexpr (T == TACO_BF16) ((__bf16*)out)[d] = (__bf16)o;
-    else ((_Float16*)out)[d] = (_Float16)o;
-    if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+    __syncthreads();
+    const int rows = min(a.group - qt * 16, 16);
+    const bool whole = n == sp.tiles;
+    // a row that began in an earlier share is this workgroup's first partial result, one that only ends later its second
+    float* leave = whole ? nullptr : a.partial + (size_t)(2 * blockIdx.x + (tile0 ? 0 : 1)) * held * (DP + 2);
+    for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
+      const int r = i / DP, d = i % DP;
+      join<T, C, DP>(a, b, h, qt, r, d, AT_WAVES, [&](int w) { return lds + (w * held + r) * (DP + 2); },
+                     leave ? leave + r * (DP + 2) : nullptr);
+    }
+    at += n;
+    in += n;
+    if (in == (uint64_t)sp.tiles * rows_per) { in = 0; ++b; }
+  }
+}
+
+// Joins the rows that cross a border of shares; one workgroup per row, `workgroups` is the first kernel's grid.
+template <int T, int C, int DP>
+__global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a, uint32_t workgroups) {
+  using A = Attend<T, C, DP>;
+  const uint32_t rows_per = a.n_heads * a.q_tiles;
+  const int b = blockIdx.x / rows_per;
+  const uint32_t row = blockIdx.x % rows_per;
+  uint32_t sum = 0, before = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) {
+    const int u = i + (threadIdx.x & 63);
+    const uint32_t t = u < a.n_seqs ? span_of(a, u, A::TT, false).tiles : 0, scan = wave_scan(t);
+    if (b >= i && b < i + 64) before = sum + (b > i ? __builtin_amdgcn_readlane(scan, b - i - 1) : 0);
+    sum += __builtin_amdgcn_readlane(scan, 63);
+  }
+  const uint64_t share = share_of(a, (uint64_t)sum * rows_per, workgroups);
+  const uint32_t tiles = span_of(a, b, A::TT, false).tiles;
+  const uint64_t start = (uint64_t)before * rows_per + (uint64_t)row * tiles, last = start + tiles - 1;
+  const uint32_t w0 = (uint32_t)(start / share), w1 = (uint32_t)(last / share);
+  if (w0 == w1) return;
+  const int held = a.group < 16 ? a.group : 16, qt = row % a.q_tiles, h = row / a.q_tiles, rows = min(a.group - qt * 16, 16);
+  for (int i = threadIdx.x; i < rows * DP; i += 256) {
+    const int r = i / DP, d = i % DP;
+    join<T, C, DP>(a, b, h, qt, r, d, (int)(w1 - w0 + 1),
+                   [&](int k) { return a.partial + ((size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r) * (DP + 2); }, nullptr);
   }
 }
 
@@ -518,45 +642,113 @@ extern "C" int taco_kv_append(const taco_kv_cache* c, const taco_kv_append_args*
   return TACO_OK;
 }
 
-extern "C" int64_t taco_kv_attend_workspace(const taco_kv_cache* c, const taco_kv_attend_args* t) {
-  const char* who = "taco_kv_attend_workspace";
-  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
-  const int rc = check_cache(c, who, t->dtype);
-  if (rc != TACO_OK) return rc;
-  return 0;
-}
-
 namespace {
 
+// Everything about a call that its sizes decide.
+struct Plan {
+  int group, q_tiles, held, dp, tt;
+  uint32_t workgroups, least;
+  int64_t bytes;
+};
+
 template <int T, int C, int DP>
-int launch_attend(const AttendParams& a, hipStream_t s) {
-  const int rows = a.group < 16 ? a.group : 16;
-  const size_t lds = (size_t)AT_WAVES * rows * (DP + 2) * 4;
-  auto kernel = taco_kv_attend_kernel<T, C, DP>;
-  if (lds > 65536) TACO_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  kernel<<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles)), dim3(64 * AT_WAVES), lds, s>>>(a);
+int plan_of(Plan& p, int device, int n_cu) {
+  // workgroups of this kernel that a CU holds: a grid beyond that would end with a part-filled round
+  static std::atomic<int> known[64][17];
+  p.tt = Attend<T, C, DP>::TT;
+  const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
+  int per_cu = known[device][p.held].load(std::memory_order_relaxed);
+  if (!per_cu) {
+    auto kernel = taco_kv_attend_kernel<T, C, DP>;
+    if (lds > 65536) TACO_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    TACO_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, 64 * AT_WAVES, lds));
+    if (per_cu < 1) TACO_FAIL(TACO_EINVAL, "taco_kv_attend: the kernel does not fit a CU");
+    known[device][p.held].store(per_cu, std::memory_order_relaxed);
+  }
+  p.workgroups = (uint32_t)(per_cu * n_cu);
+  return TACO_OK;
+}
+template <int T, int C, int DP>
+int launch_attend(const AttendParams& a, const Plan& p, hipStream_t s) {
+  const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
+  taco_kv_attend_kernel<T, C, DP><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
+  if (p.bytes) taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles)), dim3(256), 0, s>>>(a, p.workgroups);
   TACO_HIP(hipGetLastError());
   return TACO_OK;
 }
-template <int T, int C>
-int launch_attend(const AttendParams& a, hipStream_t s) {
-  if (a.head_dim <= 64) return launch_attend<T, C, 64>(a, s);
-  if (a.head_dim <= 128) return launch_attend<T, C, 128>(a, s);
-  return launch_attend<T, C, 256>(a, s);
+
+template <typename F>
+int by_types(const taco_kv_cache* c, int dtype, F&& f) {
+  const auto by_dim = [&](auto t, auto h) {
+    if (c->head_dim <= 64) return f(t, h, std::integral_constant<int, 64>());
+    if (c->head_dim <= 128) return f(t, h, std::integral_constant<int, 128>());
+    return f(t, h, std::integral_constant<int, 256>());
+  };
+  using F32 = std::integral_constant<int, TACO_F32>;
+  using F16 = std::integral_constant<int, TACO_F16>;
+  using BF16 = std::integral_constant<int, TACO_BF16>;
+  using E4M3 = std::integral_constant<int, TACO_E4M3>;
+  if (c->dtype == TACO_F32) return by_dim(F32(), F32());
+  if (c->dtype == TACO_F16) return by_dim(F16(), F16());
+  if (c->dtype == TACO_BF16) return by_dim(BF16(), BF16());
+  if (dtype == TACO_F16) return by_dim(F16(), E4M3());
+  return by_dim(BF16(), E4M3());
+}
+
+// Checks the sizes and settles the plan; the device is current.
+int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who, Plan& p) {
+  p.group = t->n_q_heads / c->n_heads;
+  p.q_tiles = (p.group + 15) / 16;
+  p.held = p.group < 16 ? p.group : 16;
+  p.dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
+  int n_cu;
+  int rc = taco_device_check(c->device, &n_cu);
+  if (rc != TACO_OK) return rc;
+  rc = by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return plan_of<ty.value, ca.value, dp.value>(p, c->device, n_cu); });
+  if (rc != TACO_OK) return rc;
+  const int64_t rows = (int64_t)t->n_seqs * c->n_heads * p.q_tiles;
+  const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
+  // a share has a tile for every wave at least; no more workgroups than that leaves work for
+  p.least = AT_WAVES;
+  const int64_t most = (rows * (tiles < 1 ? 1 : tiles) + p.least - 1) / p.least;
+  if (most < p.workgroups) p.workgroups = (uint32_t)most;
+  p.bytes = (int64_t)2 * p.workgroups * p.held * (p.dp + 2) * 4;
+  return TACO_OK;
+}
+
+int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who) {
+  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
+  const int rc = check_cache(c, who, t->dtype);
+  if (rc != TACO_OK) return rc;
+  if (t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d utterances, table width %d", who, t->n_seqs, t->table_width);
+  if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
+  if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
+  // rows and 16-token tiles are counted in 32 bits
+  if ((int64_t)t->n_seqs * t->n_q_heads >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
+    TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads and up to %d pages", who, t->n_seqs, t->n_q_heads, t->table_width);
+  return TACO_OK;
 }
 
 }  // namespace
 
+extern "C" int64_t taco_kv_attend_workspace(const taco_kv_cache* c, const taco_kv_attend_args* t) {
+  const char* who = "taco_kv_attend_workspace";
+  int rc = check_attend(c, t, who);
+  if (rc != TACO_OK) return rc;
+  if (t->n_seqs == 0) return 0;
+  DeviceScope on_device(c->device);
+  TACO_HIP(on_device.status);
+  Plan p;
+  rc = plan_attend(c, t, who, p);
+  return rc == TACO_OK ? p.bytes : rc;
+}
+
 extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, void* stream) {
   const char* who = "taco_kv_attend";
-  if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
-  int rc = check_cache(c, who, t->dtype);
+  int rc = check_attend(c, t, who);
   if (rc != TACO_OK) return rc;
-  if (t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d utterances, table width %d", who, t->n_seqs, t->table_width);
-  if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
   if (t->window < 0) TACO_FAIL(TACO_EINVAL, "%s: window %d", who, t->window);
-  if (!(t->scale == t->scale) || t->scale - t->scale != 0.0f) TACO_FAIL(TACO_EINVAL, "%s: scale is not finite", who);
-  if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
+  if (!(t->scale - t->scale == 0.0f)) TACO_FAIL(TACO_EINVAL, "%s: scale is not finite", who);
   if (t->n_seqs == 0) return TACO_OK;
   if (!t->lens || (!t->table && t->table_width)) TACO_FAIL(TACO_EINVAL, "%s: NULL table or lens", who);
   AttendParams a;
@@ -564,26 +756,20 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
   if (!(row_strides(t->q, t->q_stride, size, a.q_st) && row_strides(t->out, t->out_stride, size, a.o_st) &&
         row_strides(c->k, c->k_stride, held, a.kp_st) && row_strides(c->v, c->v_stride, held, a.vp_st)))
     TACO_FAIL(TACO_EINVAL, "%s: rows must start at multiples of 16 bytes (and not be NULL)", who);
-  a.group = t->n_q_heads / c->n_heads;
-  a.q_tiles = (a.group + 15) / 16;
-  if ((int64_t)t->n_seqs * c->n_heads * a.q_tiles >= (1ll << 31)) TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads", who, t->n_seqs, t->n_q_heads);
-  int n_cu;
   DeviceScope on_device(c->device);
   TACO_HIP(on_device.status);
-  rc = taco_device_check(c->device, &n_cu);
+  Plan p;
+  rc = plan_attend(c, t, who, p);
   if (rc != TACO_OK) return rc;
+  if (p.bytes && (!t->workspace || !aligned(t->workspace) || t->workspace_bytes < p.bytes)) TACO_FAIL(TACO_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes, has %lld", who, (long long)p.bytes, (long long)t->workspace_bytes);
   a.k_pages = (const char*)c->k; a.v_pages = (const char*)c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale;
   a.q = (const char*)t->q; a.out = (char*)t->out; a.lse = t->lse; a.table = t->table; a.lens = t->lens; a.flags = c->flags;
   a.table_stride = t->table_stride; a.page16 = taco_make_divisor((uint32_t)c->page_size / 16);
   a.scale_log2 = t->scale * 1.44269504088896340736f;
   a.n_seqs = t->n_seqs; a.table_width = t->table_width; a.n_pages = c->n_pages; a.n_heads = c->n_heads;
   a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.window = t->window;
-  hipStream_t s = (hipStream_t)stream;
-  if (c->dtype == TACO_F32) return launch_attend<TACO_F32, TACO_F32>(a, s);
-  if (c->dtype == TACO_F16) return launch_attend<TACO_F16, TACO_F16>(a, s);
-  if (c->dtype == TACO_BF16) return launch_attend<TACO_BF16, TACO_BF16>(a, s);
-  if (t->dtype == TACO_F16) return launch_attend<TACO_F16, TACO_E4M3>(a, s);
-  return launch_attend<TACO_BF16, TACO_E4M3>(a, s);
+  a.group = p.group; a.q_tiles = p.q_tiles; a.partial = (float*)t->workspace; a.least = (int)p.least;
+  return by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return launch_attend<ty.value, ca.value, dp.value>(a, p, (hipStream_t)stream); });
 }
 
 extern "C" int taco_kv_status(const taco_kv_cache* c, void* stream) {
