@@ -148,7 +148,7 @@ struct AttendParams {
   uint32_t* flags;
   int64_t table_stride;
   taco_divisor page16;                                    // 16-token blocks of a page
-  float* partial;                                    // [2 * workgroups][rows][2 + DP], see Shares
+  float* partial;                                    // the workgroups' partial results, see Partials
   float scale_log2;                                  // scale * log2(e)
   int32_t n_seqs, table_width, n_pages, n_heads, n_q_heads, group, q_tiles, head_dim, window;
   int32_t least;                                     // tiles of a workgroup's share at least
@@ -377,62 +377,80 @@ struct Attend {
 // a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
 // by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
 // kernel joins in the order of the workgroups.
-struct Span {
-  int low, len;        // seen tokens [low, len)
-  uint32_t tiles;      // of one row; an utterance that sees nothing has one, so that somebody writes its zeros
-};
-__device__ __forceinline__ Span span_of(const AttendParams& a, int b, int tt, bool flag) {
-  Span s;
-  s.len = a.lens[b];
-  const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
-  if (s.len < 0 || s.len > room) {
-    if (flag) atomicOr(a.flags, TACO_KV_BAD_PLACE);
-    s.len = s.len < 0 ? 0 : (int)room;
-  }
-  s.low = a.window > 0 ? max(0, s.len - a.window) : 0;
-  s.tiles = s.len > s.low ? (uint32_t)((s.len + tt - 1) / tt - s.low / tt) : 1;
-  return s;
+// Divisions whose operands nearly always fit 32 bits (an operand that does not is an utterance line of 2^32 tiles).
+__device__ __forceinline__ uint64_t div64(uint64_t n, uint64_t d) {
+  return (n >> 32) || (d >> 32) ? n / d : (uint64_t)((uint32_t)n / (uint32_t)d);
 }
-// Inclusive sum over the lanes of a wave.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-// Tiles of one row of every utterance, summed over the utterances (every wave for itself, 64 utterances at a time).
-__device__ __forceinline__ uint32_t all_tiles(const AttendParams& a, int tt) {
-  uint32_t sum = 0;
-  for (int i = 0; i < a.n_seqs; i += 64) {
-    const int b = i + (threadIdx.x & 63);
-    const uint32_t t = b < a.n_seqs ? span_of(a, b, tt, blockIdx.x == 0 && threadIdx.x < 64).tiles : 0;
-    sum += __builtin_amdgcn_readlane(wave_scan(t), 63);
-  }
-  return sum;
-}
-// The utterance that tile `at` (counted with one row per utterance) belongs to, and the tiles before it.
-__device__ __forceinline__ int find_utterance(const AttendParams& a, int tt, uint32_t at, uint32_t& before) {
-  uint32_t sum = 0;
-  for (int i = 0; i < a.n_seqs; i += 64) {
-    const int b = i + (threadIdx.x & 63);
-    const uint32_t t = b < a.n_seqs ? span_of(a, b, tt, false).tiles : 0, scan = wave_scan(t), all = __builtin_amdgcn_readlane(scan, 63);
-    if (at - sum < all) {
-      const int n = __popcll(__ballot(sum + scan <= at));       // utterances of this 64 that end at or before `at`
-      before = sum + (n ? __builtin_amdgcn_readlane(scan, n - 1) : 0);
-      return i + n;
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+// 64 utterances, one per lane: what each sees and how many tiles its rows have.
+template <int TT>
+struct Utterances {
+  int base;                  // the first of them
+  uint32_t before;           // tiles of one row of every utterance in front of them
+  int low, len;              // seen tokens [low, len) of this lane's utterance
+  uint32_t tiles, scan;      // tiles of one of its rows (one that sees nothing has one, so that somebody writes its zeros); inclusive sum
+
+  __device__ __forceinline__ void load(const AttendParams& a, int first, bool flag) {
+    base = first;
+    const int b = first + (threadIdx.x & 63);
+    len = low = 0;
+    tiles = 0;
+    if (b < a.n_seqs) {
+      len = a.lens[b];
+      const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
+      if (len < 0 || len > room) {
+        if (flag) atomicOr(a.flags, TACO_KV_BAD_PLACE);
+        len = len < 0 ? 0 : (int)room;
+      }
+      low = a.window > 0 ? max(0, len - a.window) : 0;
+      tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
     }
-    sum += all;
+    scan = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t u = __shfl_up(scan, d, 64);
+      if ((int)(threadIdx.x & 63) >= d) scan += u;
+    }
   }
-  before = sum;
-  return a.n_seqs;
-}
+  // Loads the first 64 and sums the tiles of all.
+  __device__ __forceinline__ uint32_t load_all(const AttendParams& a, bool flag) {
+    uint32_t sum = 0;
+    for (int i = 64; i < a.n_seqs; i += 64) {
+      load(a, i, flag);
+      sum += lane_of(scan, 63);
+    }
+    load(a, 0, flag);
+    before = 0;
+    return sum + lane_of(scan, 63);
+  }
+  // Moves on to the 64 that utterance `b` is one of.
+  __device__ __forceinline__ void move_to(const AttendParams& a, int b) {
+    while (b >= base + 64) {
+      before += lane_of(scan, 63);
+      load(a, base + 64, false);
+    }
+  }
+  // Moves on to the 64 in which tile `at` lies (one row per utterance counted) and returns its utterance.
+  __device__ __forceinline__ int find(const AttendParams& a, uint32_t at) {
+    while (at - before >= lane_of(scan, 63)) move_to(a, base + 64);
+    return base + __popcll(__ballot(before + scan <= at));      // those that end at or before it
+  }
+  __device__ __forceinline__ uint32_t before_of(int b) const { return before + lane_of(scan, b - base) - lane_of(tiles, b - base); }
+};
+
 __device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all, uint32_t workgroups) {
-  const uint64_t share = (all + workgroups - 1) / workgroups;
+  const uint64_t share = div64(all + workgroups - 1, workgroups);
   return share < (uint64_t)a.least ? (uint64_t)a.least : share;
 }
+
+// Partial results: first the maxima and sums of all of them, [2 per workgroup][queries][2], then the outputs [..][DP].
+template <int DP>
+struct Partials {
+  float *ml, *o;
+  __device__ __forceinline__ Partials(const AttendParams& a, uint32_t workgroups, int held)
+      : ml(a.partial), o(a.partial + (((size_t)workgroups * held * 4 + 3) & ~(size_t)3)) {}
+};
 
 template <int T>
 __device__ __forceinline__ void store_out(char* row, int d, float o) {
@@ -440,29 +458,16 @@ __device__ __forceinline__ void store_out(char* row, int d, float o) {
   else if constexpr (T == TACO_BF16) ((__bf16*)row)[d] = (__bf16)o;
   else ((_Float16*)row)[d] = (_Float16)o;
 }
-// Element d of query r of a row from `n` partial results part(i): final, or partial again where `leave` is given.
-template <int T, int C, int DP, typename Part>
-__device__ __forceinline__ void join(const AttendParams& a, int b, int h, int qt, int r, int d, int n, Part part, float* leave) {
-  float m = NEG_INF;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, part(i)[0]);
-  float sum = 0.0f, o = 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const float* p = part(i);
-    const float f = p[0] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(p[0] - m);
-    sum += f * p[1];
-    o += f * p[2 + d];
-  }
-  if (leave) {
-    if (d == 0) { leave[0] = m; leave[1] = sum; }
-    leave[2 + d] = o;
-    return;
-  }
+// Element d of a finished row: o and `sum` are relative to the maximum m.
+template <int T, int C>
+__device__ __forceinline__ void finish(const AttendParams& a, int b, int head, int h, int d, float o, float sum, float m) {
   if (d >= a.head_dim) return;
-  const int head = h * a.group + qt * 16 + r;
   o = sum == 0.0f ? 0.0f : o / sum * (C == TACO_E4M3 ? a.v_scale[h] : 1.0f);
   store_out<T>(a.out + (int64_t)b * a.o_st[0] + (int64_t)head * a.o_st[1], d, o);
   if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
 }
+// What a part counts for beside the common maximum.
+__device__ __forceinline__ float weight_of(float m_part, float m) { return m_part == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_part - m); }
 
 template <int T, int C, int DP>
 __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const AttendParams a) {
@@ -470,19 +475,21 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
-  const uint64_t all = (uint64_t)all_tiles(a, A::TT) * rows_per, share = share_of(a, all, gridDim.x);
+  Utterances<A::TT> us;
+  const uint64_t all = (uint64_t)us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64) * rows_per, share = share_of(a, all, gridDim.x);
   uint64_t at = share * blockIdx.x;
   const uint64_t end = at + share < all ? at + share : all;
   if (at >= end) return;
-  uint32_t before;
-  int b = find_utterance(a, A::TT, (uint32_t)(at / rows_per), before);
+  int b = us.find(a, (uint32_t)div64(at, rows_per));
   const int held = a.group < 16 ? a.group : 16;            // queries of a row in LDS and in the partial results
   bool first = true;
-  uint64_t in = at - (uint64_t)before * rows_per;          // tile within the utterance
+  uint64_t in = at - (uint64_t)us.before_of(b) * rows_per;     // tile within the utterance
   while (at < end) {
-    const Span sp = span_of(a, b, A::TT, false);
-    const uint32_t row = (uint32_t)(in / sp.tiles), tile0 = (uint32_t)(in - (uint64_t)row * sp.tiles);
-    const uint32_t n = (uint32_t)(end - at < sp.tiles - tile0 ? end - at : sp.tiles - tile0);
+    us.move_to(a, b);
+    const int low = (int)lane_of(us.low, b - us.base), len = (int)lane_of(us.len, b - us.base);
+    const uint32_t tiles = lane_of(us.tiles, b - us.base);
+    const uint32_t row = (uint32_t)div64(in, tiles), tile0 = (uint32_t)(in - (uint64_t)row * tiles);
+    const uint32_t n = (uint32_t)(end - at < tiles - tile0 ? end - at : tiles - tile0);
     const int qt = row % a.q_tiles, h = row / a.q_tiles;
     taco_u4 q[A::NQ];
     A::load_q(a, b, h, qt, q);
@@ -493,9 +500,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     for (int blk = 0; blk < A::NB; ++blk)
 #pragma unroll
       for (int e = 0; e < A::VE; ++e) st.o[blk][e] = taco_f4{0, 0, 0, 0};
-    const int base = (sp.low / A::TT + (int)tile0) * A::TT;
-    if (sp.len > sp.low)
-      for (uint32_t t = wave; t < n; t += AT_WAVES) A::tile(a, b, h, base + (int)t * A::TT, sp.low, sp.len, factor, q, st);
+    const int base = (low / A::TT + (int)tile0) * A::TT;
+    if (len > low)
+      for (uint32_t t = wave; t < n; t += AT_WAVES) A::tile(a, b, h, base + (int)t * A::TT, low, len, factor, q, st);
     // join the waves: [wave][query][m, l, DP outputs]
     if (!first) __syncthreads();
     first = false;
@@ -512,44 +519,93 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     }
     __syncthreads();
     const int rows = min(a.group - qt * 16, 16);
-    const bool whole = n == sp.tiles;
     // a row that began in an earlier share is this workgroup's first partial result, one that only ends later its second
-    float* leave = whole ? nullptr : a.partial + (size_t)(2 * blockIdx.x + (tile0 ? 0 : 1)) * held * (DP + 2);
+    const Partials<DP> parts(a, gridDim.x, held);
+    const size_t slot = (size_t)(2 * blockIdx.x + (tile0 ? 0 : 1)) * held;
     for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
       const int r = i / DP, d = i % DP;
-      join<T, C, DP>(a, b, h, qt, r, d, AT_WAVES, [&](int w) { return lds + (w * held + r) * (DP + 2); },
-                     leave ? leave + r * (DP + 2) : nullptr);
+      const float* p = lds + r * (DP + 2);
+      float m = NEG_INF, sum = 0.0f, o = 0.0f;
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) m = fmaxf(m, p[w * held * (DP + 2)]);
+#pragma unroll
+      for (int w = 0; w < AT_WAVES; ++w) {
+        const float* x = p + w * held * (DP + 2);
+        const float f = weight_of(x[0], m);
+        sum += f * x[1];
+        o += f * x[2 + d];
+      }
+      if (n == tiles) {
+        finish<T, C>(a, b, h * a.group + qt * 16 + r, h, d, o, sum, m);
+      } else {
+        if (d == 0) { parts.ml[(slot + r) * 2] = m; parts.ml[(slot + r) * 2 + 1] = sum; }
+        parts.o[(slot + r) * DP + d] = o;
+      }
     }
     at += n;
     in += n;
-    if (in == (uint64_t)sp.tiles * rows_per) { in = 0; ++b; }
+    if (in == (uint64_t)tiles * rows_per) { in = 0; ++b; }
   }
 }
 
-// Joins the rows that cross a border of shares; one workgroup per row, `workgroups` is the first kernel's grid.
+// Joins the rows that cross a border of shares: one workgroup per row and query, `workgroups` is the first kernel's grid.  A
+// long utterance alone leaves a hundred parts of a row, so the maxima are taken by 256 threads at a time and the outputs by as many
+// groups of DP / 4 threads as there are, each with its own parts, in a fixed order.
 template <int T, int C, int DP>
 __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a, uint32_t workgroups) {
   using A = Attend<T, C, DP>;
+  constexpr int GROUPS = 256 / (DP / 4);
+  __shared__ float red[2][4], weight[256];
+  __shared__ taco_f4 outs[GROUPS][DP / 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t rows_per = a.n_heads * a.q_tiles;
-  const int b = blockIdx.x / rows_per;
-  const uint32_t row = blockIdx.x % rows_per;
-  uint32_t sum = 0, before = 0;
-  for (int i = 0; i < a.n_seqs; i += 64) {
-    const int u = i + (threadIdx.x & 63);
-    const uint32_t t = u < a.n_seqs ? span_of(a, u, A::TT, false).tiles : 0, scan = wave_scan(t);
-    if (b >= i && b < i + 64) before = sum + (b > i ? __builtin_amdgcn_readlane(scan, b - i - 1) : 0);
-    sum += __builtin_amdgcn_readlane(scan, 63);
+  const int held = a.group < 16 ? a.group : 16, r = blockIdx.x % held;
+  const uint32_t nth = blockIdx.x / held, row = nth % rows_per;
+  const int b = nth / rows_per, qt = row % a.q_tiles, h = row / a.q_tiles;
+  if (qt * 16 + r >= a.group) return;
+  Utterances<A::TT> us;
+  const uint64_t share = share_of(a, (uint64_t)us.load_all(a, false) * rows_per, workgroups);
+  us.move_to(a, b);
+  const uint32_t tiles = lane_of(us.tiles, b - us.base);
+  const uint64_t start = (uint64_t)us.before_of(b) * rows_per + (uint64_t)row * tiles, last = start + tiles - 1;
+  const uint32_t w0 = (uint32_t)div64(start, share), n = (uint32_t)div64(last, share) - w0 + 1;
+  if (n == 1) return;
+  const Partials<DP> parts(a, workgroups, held);
+  const auto at = [&](uint32_t k) { return (size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r; };
+  float m = NEG_INF;
+  for (uint32_t k = tid; k < n; k += 256) m = fmaxf(m, parts.ml[at(k) * 2]);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+  if (lane == 0) red[0][wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float sum = 0.0f;
+  taco_f4 o = {0, 0, 0, 0};
+  const int mine = tid / (DP / 4), piece = tid % (DP / 4);
+  for (uint32_t k0 = 0; k0 < n; k0 += 256) {
+    if (k0) __syncthreads();
+    const uint32_t k = k0 + tid;
+    if (k < n) {
+      const float f = weight_of(parts.ml[at(k) * 2], m);
+      weight[tid] = f;
+      sum += f * parts.ml[at(k) * 2 + 1];
+    }
+    __syncthreads();
+    const uint32_t here = n - k0 < 256 ? n - k0 : 256;
+#pragma unroll 4
+    for (uint32_t j = mine; j < here; j += GROUPS) o += weight[j] * *(const taco_f4*)(parts.o + at(k0 + j) * DP + piece * 4);
   }
-  const uint64_t share = share_of(a, (uint64_t)sum * rows_per, workgroups);
-  const uint32_t tiles = span_of(a, b, A::TT, false).tiles;
-  const uint64_t start = (uint64_t)before * rows_per + (uint64_t)row * tiles, last = start + tiles - 1;
-  const uint32_t w0 = (uint32_t)(start / share), w1 = (uint32_t)(last / share);
-  if (w0 == w1) return;
-  const int held = a.group < 16 ? a.group : 16, qt = row % a.q_tiles, h = row / a.q_tiles, rows = min(a.group - qt * 16, 16);
-  for (int i = threadIdx.x; i < rows * DP; i += 256) {
-    const int r = i / DP, d = i % DP;
-    join<T, C, DP>(a, b, h, qt, r, d, (int)(w1 - w0 + 1),
-                   [&](int k) { return a.partial + ((size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r) * (DP + 2); }, nullptr);
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  if (lane == 0) red[1][wave] = sum;
+  outs[mine][piece] = o;
+  __syncthreads();
+  sum = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+  for (int d = tid; d < DP; d += 256) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) total += outs[i][d / 4][d % 4];
+    finish<T, C>(a, b, h * a.group + qt * 16 + r, h, d, total, sum, m);
   }
 }
 
@@ -672,7 +728,7 @@ template <int T, int C, int DP>
 int launch_attend(const AttendParams& a, const Plan& p, hipStream_t s) {
   const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
   taco_kv_attend_kernel<T, C, DP><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
-  if (p.bytes) taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles)), dim3(256), 0, s>>>(a, p.workgroups);
+  if (p.bytes) taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a, p.workgroups);
   TACO_HIP(hipGetLastError());
   return TACO_OK;
 }
@@ -712,7 +768,7 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char
   p.least = AT_WAVES;
   const int64_t most = (rows * (tiles < 1 ? 1 : tiles) + p.least - 1) / p.least;
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
-  p.bytes = (int64_t)2 * p.workgroups * p.held * (p.dp + 2) * 4;
+  p.bytes = ((int64_t)p.workgroups * p.held * 4 + 3) / 4 * 16 + (int64_t)2 * p.workgroups * p.held * p.dp * 4;
   return TACO_OK;
 }
 
@@ -724,7 +780,7 @@ int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const cha
   if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
   if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
   // rows and 16-token tiles are counted in 32 bits
-  if ((int64_t)t->n_seqs * t->n_q_heads >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
+  if ((int64_t)t->n_seqs * (t->n_q_heads + 16ll * c->n_heads) >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
     TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads and up to %d pages", who, t->n_seqs, t->n_q_heads, t->table_width);
   return TACO_OK;
 }
