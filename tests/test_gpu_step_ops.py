@@ -547,18 +547,18 @@ def make_codes(n, k, group, scale_dtype, zeros, g):
 
 
 def check_matvec(codes, scales, zeros, group, bias, x, got):
-  """A group's sum of c x in fp32 is off by at most (group + 8) U of the sum of |terms|; taking the offset off and
-  scaling adds a few U more, the groups' and the waves' sums (groups + 16) U.  The terms are (c - z) x for fp32 and float16,
-  (128 + c) x and (128 + z) sum x for bfloat16; then the bias and one rounding."""
+  """A group's sum in fp32 is off by at most 3 (group + 8) U of the sum of |terms|; taking the offset off and
+  scaling adds a few U more, the groups' and the waves' sums (groups + 16) U.  The terms are (16 + c) x and (16 + z) sum x, x in three parts for fp32 (whose sums of |terms| are together at most 1.01 times
+  as large); then the bias and one rounding."""
   n, k = codes.shape
   s = scales.double().repeat_interleave(group, 1)[:, :k]
   z = torch.full_like(s, 8.0) if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
   c, x64 = codes.double(), x.double()
   want = x64 @ ((c - z) * s).t()
-  size = (256 + c + z if x.dtype == BF16 else (c - z).abs()) * s
+  size = 1.01 * (32 + c + z) * s
   if bias is not None:
     want = want + bias.double()
-  slack = (group + 8 + scales.shape[1] + 16 + 8) * U * (x64.abs() @ size.t()) + 2 * U * want.abs()
+  slack = (3 * (group + 8) + scales.shape[1] + 16 + 8) * U * (x64.abs() @ size.t()) + 2 * U * want.abs()
   tol = slack + half_step(x.dtype) * (want.abs() + slack) + (2.0 ** -25 if x.dtype == F16 else 0)
   excess = (got.double() - want).abs() - tol
   assert excess.max().item() <= 0, (excess.max().item(), want.flatten()[excess.argmax()].item())
@@ -580,6 +580,13 @@ MATVECS = [
   (BF16, F16, 16, 130, 1000, 64, False, False),
   (BF16, BF16, 130, 50, 65, 32, False, True),
   (BF16, BF16, 1, 3, 20000, 128, True, False),
+  # every way of dividing the rows: up to a row block per CU, two, four
+  (F32, F16, 2, 4100, 200, 32, True, True),
+  (F16, F16, 16, 6000, 257, 64, False, False),
+  (BF16, F32, 1, 9000, 300, 32, True, False),
+  (BF16, BF16, 7, 8200, 2500, 128, True, True),
+  (F32, F32, 16, 8209, 160, 64, False, True),
+  (F16, F16, 20, 9001, 130, 32, False, False),
 ]
 
 
@@ -618,9 +625,9 @@ def test_matvec_extreme_codes_and_values():
         x = torch.full((1, 64), v, dtype=dtype, device=DEV)
         x[0, ::3] *= -1
         got = W.matvec(x)
-        size = (256 + code + zero if dtype == BF16 else abs(code - zero)) * 1e-3 * x.double().abs().sum().item()
+        size = 1.01 * (32 + code + zero) * 1e-3 * x.double().abs().sum().item()
         want = (code - zero) * scales[0].double() * x.double().sum()
-        tol = 110 * U * size + half_step(dtype) * want.abs() + {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
+        tol = 250 * U * size + half_step(dtype) * want.abs() + {F16: 2.0 ** -25, BF16: 2.0 ** -126, F32: 2.0 ** -126}[dtype]
         assert ((got.double() - want).abs() <= tol).all(), (dtype, code, zero, v)
 
 

@@ -141,11 +141,11 @@ def _qmat(**change):
 
 
 def test_size_of_a_packed_matrix():
-  """Blocks of 16 x 128 codes (1 KiB), then 16 scales, then 16 zero points per block row and group."""
+  """Blocks of 16 x 128 codes (1 KiB) for whole multiples of 64 rows, then 64 scales, then 64 zero points per 64 rows and group."""
   L = _lib.lib()
   for n, k, group, dtype, zeros, want in (
-    (32, 100, 64, abi.TACO_F16, 0, 2 * 1024 + 2 * 2 * 32), (32, 100, 64, abi.TACO_F16, 1, 2 * 1024 + 2 * 2 * 32 + 2 * 2 * 16),
-    (1, 1, 32, abi.TACO_F32, 0, 1024 + 4 * 64), (17, 129, 128, abi.TACO_BF16, 1, 4 * 1024 + 4 * 32 + 4 * 16),
+    (32, 100, 64, abi.TACO_F16, 0, 4 * 1024 + 2 * 2 * 64), (32, 100, 64, abi.TACO_F16, 1, 4 * 1024 + 2 * 2 * 64 + 2 * 64),
+    (1, 1, 32, abi.TACO_F32, 0, 4 * 1024 + 4 * 4 * 64), (65, 129, 128, abi.TACO_BF16, 1, 16 * 1024 + 2 * 4 * 64 + 4 * 64),
     (28672, 8192, 128, abi.TACO_BF16, 0, 28672 * 4096 + 28672 * 64 * 2),
     (1 << 20, 1 << 20, 128, abi.TACO_F32, 0, (1 << 39) + (1 << 35))):
     assert L.taco_qmat_bytes(C.byref(_qmat(n_rows=n, n_cols=k, group=group, scale_dtype=dtype, has_zeros=zeros))) == want
