@@ -10,6 +10,8 @@ import os
 import subprocess
 from typing import Optional
 
+import torch
+
 from tacotron_amd import abi
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
@@ -70,8 +72,9 @@ def lib() -> C.CDLL:
   L.taco_last_decode_timing.argtypes = [vp, C.POINTER(C.c_double), C.POINTER(i32)]
   L.taco_set_frame_clock.argtypes = [vp, vp, i32]
   L.taco_set_precision.argtypes = [vp, i32]
-  L.taco_kv_append.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAppendArgs), vp]
-  L.taco_kv_attend.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAttendArgs), vp]
+  # the argument blocks are passed as pointers to structs or as their bytes
+  L.taco_kv_append.argtypes = [C.POINTER(abi.TacoKvCache), vp, vp]
+  L.taco_kv_attend.argtypes = [C.POINTER(abi.TacoKvCache), vp, vp]
   L.taco_kv_attend_workspace.argtypes = [C.POINTER(abi.TacoKvCache), C.POINTER(abi.TacoKvAttendArgs)]
   L.taco_kv_attend_workspace.restype = C.c_int64
   L.taco_kv_status.argtypes = [C.POINTER(abi.TacoKvCache), vp]
@@ -99,6 +102,11 @@ class TacoTimeoutError(TacoError, TimeoutError):
 
 
 _ERROR_TYPES = {ERANGE: TacoIndexError, ETIMEDOUT: TacoTimeoutError}
+
+
+def raw_stream(device_index: int) -> int:
+  """The device's current stream as the pointer the C ABI takes."""
+  return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def check(rc: int) -> None:

@@ -9,11 +9,22 @@ the device can see - a table entry that is no page, a length beyond the table - 
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple, Union
+import struct
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 
 from tacotron_amd import _lib, abi
+
+
+# A call's argument block is its addresses, packed here, followed by what its tensors' forms say, kept per form.
+_APPEND_POINTERS = struct.Struct("8Q")      # k, v, q, q_out, table, past, offsets, inv_freq
+_ATTEND_POINTERS = struct.Struct("6Q")      # q, out, lse, table, lens, workspace
+_MOST_FORMS = 256
+
+
+def _form(t: torch.Tensor) -> Tuple:
+  return t.shape, t.stride(), t.dtype, t.device
 
 
 def _device(device: Union[torch.device, str, int]) -> torch.device:
@@ -93,6 +104,9 @@ class PagedCache:
     self._ref = C.byref(self._c)
     self._takes = (torch.float16, torch.bfloat16) if k.dtype == torch.float8_e4m3fn else (k.dtype,)
     self._lib = _lib.lib()
+    # what a call's checks have found, by the shapes, strides, types and devices of its tensors (never by their addresses)
+    self._append_forms: Dict[Tuple, bytes] = {}
+    self._attend_forms: Dict[Tuple, Tuple[bytes, int]] = {}
 
   @property
   def n_pages(self) -> int:
@@ -110,30 +124,21 @@ class PagedCache:
   def head_dim(self) -> int:
     return self.k.shape[3]
 
-  def _stream(self) -> int:
-    return torch.cuda.current_stream(self.device).cuda_stream
-
-  def _rows(self, t: torch.Tensor, name: str, tokens: int, heads: Optional[int]) -> torch.Tensor:
-    """``t`` [tokens, heads, head_dim] checked, as the kernels can read it (a copy where its rows are not aligned)."""
+  def _rows(self, t: torch.Tensor, name: str, tokens: int, heads: Optional[int]) -> None:
     shape = t.shape
     if len(shape) != 3 or shape[0] != tokens or shape[2] != self.head_dim or (shape[1] != heads if heads else shape[1] < 1):
       raise ValueError(f"{name} must be [{tokens}, {heads or 'heads'}, {self.head_dim}], got {tuple(shape)}")
     if t.dtype not in self._takes or t.device != self.device:
       raise ValueError(f"{name} must be {' or '.join(str(d) for d in self._takes)} on {self.device}, got {t.dtype} on {t.device}")
-    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
 
-  def _out(self, out: Optional[torch.Tensor], like: torch.Tensor) -> torch.Tensor:
-    if out is None:
-      return torch.empty(like.shape, dtype=like.dtype, device=self.device)
+  def _out(self, out: torch.Tensor, like: torch.Tensor) -> None:
     if out.shape != like.shape or out.dtype != like.dtype or out.device != self.device or not _rows_ok(out):
       raise ValueError(f"out must be {like.dtype} {tuple(like.shape)} on {self.device} with unit stride and rows at multiples of "
                        f"16 bytes, got {out.dtype} {tuple(out.shape)} on {out.device}")
-    return out
 
-  def _index(self, t: torch.Tensor, name: str, size: int) -> int:
+  def _index(self, t: torch.Tensor, name: str, size: int) -> None:
     if t.dtype != torch.int32 or t.shape != (size,) or t.device != self.device or not t.is_contiguous():
       raise ValueError(f"{name} must be a contiguous int32 [{size}] tensor on {self.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
 
   def _table(self, table: torch.Tensor) -> Tuple[int, int]:
     if table.dtype != torch.int32 or table.dim() != 2 or table.device != self.device:
@@ -154,36 +159,63 @@ class PagedCache:
     tokens, rotated likewise: returned, or written to ``out`` (which may be ``q``).  Rows that belong to no utterance are
     left as they were in ``out``.  No two tokens of a call may go to the same place, and ``out`` may overlap no other
     input."""
+    key = (_form(k), _form(v), _form(table), _form(past), None if q is None else _form(q), None if offsets is None else _form(offsets),
+           None if inv_freq is None else _form(inv_freq), interleaved, None if out is None else _form(out))
+    tail = self._append_forms.get(key)
+    kp, vp, qp = k.data_ptr(), v.data_ptr(), 0 if q is None else q.data_ptr()
+    op = 0 if out is None else out.data_ptr()
+    if tail is None or (kp | vp | qp | op) % 16:
+      rows = [None if t is None else t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format) for t in (k, v, q)]
+      tail = self._append_tail(rows[0], rows[1], table, past, rows[2], offsets, inv_freq, interleaved, out)
+      if rows[0] is k and rows[1] is v and rows[2] is q:
+        if len(self._append_forms) >= _MOST_FORMS:
+          self._append_forms.clear()
+        self._append_forms[key] = tail
+      k, v = rows[0], rows[1]      # kept until the call is enqueued
+      kp, vp, qp = k.data_ptr(), v.data_ptr(), 0 if q is None else rows[2].data_ptr()
+    if q is not None and out is None:
+      out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+      op = out.data_ptr()
+    if kp:      # no tokens have no address
+      head = _APPEND_POINTERS.pack(kp, vp, qp, op, table.data_ptr(), past.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+                                   0 if inv_freq is None else inv_freq.data_ptr())
+      rc = self._lib.taco_kv_append(self._ref, head + tail, _lib.raw_stream(self._c.device))
+      if rc:
+        _lib.check(rc)
+    return out
+
+  def _append_tail(self, k, v, table, past, q, offsets, inv_freq, interleaved, out) -> bytes:
+    """Checks an append's tensors and returns the part of its argument block that their forms decide."""
     n, width = self._table(table)
-    k, v = self._rows(k, "k", k.shape[0], self.n_heads), self._rows(v, "v", k.shape[0], self.n_heads)
+    self._rows(k, "k", k.shape[0] if k.dim() else -1, self.n_heads)
+    self._rows(v, "v", k.shape[0], self.n_heads)
     tokens = k.shape[0]
     if offsets is None and tokens != n:
       raise ValueError(f"{tokens} tokens for {n} utterances need offsets")
-    a = abi.TacoKvAppendArgs(
-      k=k.data_ptr(), v=v.data_ptr(), table=table.data_ptr(), past=self._index(past, "past", n),
-      k_stride=k.stride()[:2], v_stride=v.stride()[:2], table_stride=table.stride(0), n_tokens=tokens, n_seqs=n,
-      table_width=width, interleaved=bool(interleaved), dtype=abi.DTYPES[k.dtype])
-    if offsets is not None:
-      a.offsets = self._index(offsets, "offsets", n + 1)
     if v.dtype != k.dtype:
       raise ValueError(f"k and v differ in type: {k.dtype}, {v.dtype}")
+    self._index(past, "past", n)
+    if offsets is not None:
+      self._index(offsets, "offsets", n + 1)
+    a = abi.TacoKvAppendArgs(
+      k_stride=k.stride()[:2], v_stride=v.stride()[:2], table_stride=table.stride(0), n_tokens=tokens, n_seqs=n,
+      table_width=width, interleaved=bool(interleaved), dtype=abi.DTYPES[k.dtype])
     if inv_freq is not None:
       if inv_freq.dim() != 1 or inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > self.head_dim:
         raise ValueError(f"inv_freq must have a multiple of 8 frequencies, at most head_dim / 2 = {self.head_dim // 2}, got {tuple(inv_freq.shape)}")
       _check_vector(inv_freq, "inv_freq", torch.float64, inv_freq.shape[0], self.device)
-      a.inv_freq, a.rot_dim = inv_freq.data_ptr(), 2 * inv_freq.shape[0]
+      a.rot_dim = 2 * inv_freq.shape[0]
     if q is not None:
-      rows = self._rows(q, "q", tokens, None)
+      self._rows(q, "q", tokens, None)
       if q.dtype != k.dtype:
         raise ValueError(f"q and k differ in type: {q.dtype}, {k.dtype}")
-      out = self._out(out, q)
-      a.q, a.q_out, a.n_q_heads = rows.data_ptr(), out.data_ptr(), q.shape[1]
-      a.q_stride, a.q_out_stride = rows.stride()[:2], out.stride()[:2]
+      if out is not None:
+        self._out(out, q)
+      a.n_q_heads, a.q_stride = q.shape[1], q.stride()[:2]
+      a.q_out_stride = (q.shape[1] * q.shape[2], q.shape[2]) if out is None else out.stride()[:2]
     elif out is not None:
       raise ValueError("out without q")
-    if tokens:
-      _lib.check(self._lib.taco_kv_append(self._ref, C.byref(a), self._stream()))
-    return out
+    return bytes(a)[_APPEND_POINTERS.size:]
 
   def attend(self, q: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, scale: Optional[float] = None, window: int = 0,
              return_lse: bool = False, out: Optional[torch.Tensor] = None):
@@ -193,33 +225,55 @@ class PagedCache:
     ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
     (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
     infinite value that is seen gives NaN."""
+    key = (_form(q), _form(table), _form(lens), scale, window, None if out is None else _form(out))
+    found = self._attend_forms.get(key)
+    qp, op = q.data_ptr(), 0 if out is None else out.data_ptr()
+    if found is None or (qp | op) % 16:
+      rows = q if _rows_ok(q) else q.clone(memory_format=torch.contiguous_format)
+      found = self._attend_tail(rows, table, lens, scale, window, out)
+      if rows is q:
+        if len(self._attend_forms) >= _MOST_FORMS:
+          self._attend_forms.clear()
+        self._attend_forms[key] = found
+      q = rows      # kept until the call is enqueued
+      qp = q.data_ptr()
+    tail, need = found
+    if out is None:
+      out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+      op = out.data_ptr()
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
+    if op:        # no utterances have no address
+      # allocated per call: the allocator orders its reuse by stream, and a captured graph gets one of its own
+      work = torch.empty(need, dtype=torch.uint8, device=self.device)
+      head = _ATTEND_POINTERS.pack(qp, op, 0 if lse is None else lse.data_ptr(), table.data_ptr(), lens.data_ptr(), work.data_ptr())
+      rc = self._lib.taco_kv_attend(self._ref, head + tail, _lib.raw_stream(self._c.device))
+      if rc:
+        _lib.check(rc)
+    return (out, lse) if return_lse else out
+
+  def _attend_tail(self, q, table, lens, scale, window, out) -> Tuple[bytes, int]:
+    """Checks an attend's tensors; the part of its argument block that their forms decide, and its workspace."""
     n, width = self._table(table)
-    rows = self._rows(q, "q", n, None)
+    self._rows(q, "q", n, None)
     heads = q.shape[1]
     if heads % self.n_heads:
       raise ValueError(f"{heads} query heads cannot share {self.n_heads} cache heads evenly")
     if window < 0:
       raise ValueError(f"window must not be negative, got {window}")
-    out = self._out(out, q)
-    lse = torch.empty(n, heads, dtype=torch.float32, device=self.device) if return_lse else None
+    self._index(lens, "lens", n)
+    if out is not None:
+      self._out(out, q)
     a = abi.TacoKvAttendArgs(
-      q=rows.data_ptr(), out=out.data_ptr(), table=table.data_ptr(), lens=self._index(lens, "lens", n),
-      q_stride=rows.stride()[:2], out_stride=out.stride()[:2], table_stride=table.stride(0),
-      scale=self.head_dim ** -0.5 if scale is None else scale, window=window, n_seqs=n, table_width=width, n_q_heads=heads,
-      dtype=abi.DTYPES[q.dtype])
-    if return_lse:
-      a.lse = lse.data_ptr()
-    if n:
-      need = self._lib.taco_kv_attend_workspace(self._ref, C.byref(a))
-      if need < 0:
-        _lib.check(int(need))
-      if need:      # allocated per call: the allocator orders its reuse by stream, and a captured graph gets one of its own
-        work = torch.empty(need, dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-      _lib.check(self._lib.taco_kv_attend(self._ref, C.byref(a), self._stream()))
-    return (out, lse) if return_lse else out
+      q_stride=q.stride()[:2], out_stride=(heads * self.head_dim, self.head_dim) if out is None else out.stride()[:2],
+      table_stride=table.stride(0), scale=self.head_dim ** -0.5 if scale is None else scale, window=window, n_seqs=n,
+      table_width=width, n_q_heads=heads, dtype=abi.DTYPES[q.dtype])
+    need = self._lib.taco_kv_attend_workspace(self._ref, C.byref(a))
+    if need < 0:
+      _lib.check(int(need))
+    a.workspace_bytes = need
+    return bytes(a)[_ATTEND_POINTERS.size:], need
 
   def check(self) -> None:
     """Waits for the current stream and raises an IndexError if a call since the last check has met a table entry that is
     no page of the cache, or a position or length outside its table (such tokens are neither stored nor seen)."""
-    _lib.check(self._lib.taco_kv_status(self._ref, self._stream()))
+    _lib.check(self._lib.taco_kv_status(self._ref, _lib.raw_stream(self._c.device)))

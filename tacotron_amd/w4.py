@@ -3,7 +3,7 @@ entry points (include/taco.h).  The reference has no counterpart: it computes wi
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -66,6 +66,8 @@ class W4Matrix:
     self._ref = C.byref(c)
     self.device, self.in_features, self.out_features, self.group = packed.device, c.n_cols, c.n_rows, c.group
     self._lib = _lib.lib()
+    # vectors, row strides and result of a call, by the shapes, strides, types and devices of its tensors
+    self._forms: Dict[Tuple, Tuple] = {}
 
   @classmethod
   def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
@@ -121,24 +123,43 @@ class W4Matrix:
   def matvec(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x W^T + bias for vectors ``x`` [..., in_features] in float32, float16 or bfloat16; the result [..., out_features] has
     x's type, its sums are fp32 and rounded once.  Meant for a few vectors (the matrix is read once for every 64)."""
-    shape, dtype = x.shape, x.dtype
-    if dtype not in _FLOATS or x.device != self.device or len(shape) < 1 or shape[-1] != self.in_features:
-      raise ValueError(f"x must be a float [..., {self.in_features}] tensor on {self.device}, got {dtype} {tuple(shape)} on {x.device}")
-    if len(shape) != 2:
-      x = x.reshape(-1, self.in_features)
-    x = _rows(x)
-    n = x.shape[0]
-    want = (*shape[:-1], self.out_features)
+    key = (x.shape, x.stride(), x.dtype, x.device) if out is None else \
+          (x.shape, x.stride(), x.dtype, x.device, out.shape, out.stride(), out.dtype, out.device)
+    form = self._forms.get(key)
+    if form is None:
+      form = self._form(x, out)
+      if len(self._forms) >= 256:
+        self._forms.clear()
+      self._forms[key] = form
+    n, x_pitch, y_pitch, code, want, copies = form
+    if copies:        # columns apart, expanded or overlapping vectors
+      x = x.contiguous()
     if out is None:
-      out = torch.empty(want, dtype=dtype, device=self.device)
-    elif out.shape != want or out.dtype != dtype or out.device != self.device or (out.dim() != 2 and not out.is_contiguous()) or \
-        (out.shape[-1] > 1 and out.stride(-1) != 1) or (n > 1 and out.dim() == 2 and out.stride(0) < self.out_features):
-      raise ValueError(f"out must be {dtype} {want} on {self.device}, its rows side by side, got {out.dtype} {tuple(out.shape)} "
-                       f"{out.stride()} on {out.device}")
+      out = torch.empty(want, dtype=x.dtype, device=self.device)
     if n:
-      if n > 1 and x.stride(0) < self.in_features:      # expanded or overlapping vectors
-        x = x.contiguous()
-      _lib.check(self._lib.taco_qmat_multiply(
-        self._ref, x.data_ptr(), x.stride(0), out.data_ptr(), out.stride(0) if len(shape) == 2 else self.out_features, n,
-        abi.DTYPES[dtype], torch.cuda.current_stream(self.device).cuda_stream))
+      rc = self._lib.taco_qmat_multiply(self._ref, x.data_ptr(), x_pitch, out.data_ptr(), y_pitch, n, code,
+                                        _lib.raw_stream(self._c.device))
+      if rc:
+        _lib.check(rc)
     return out
+
+  def _form(self, x: torch.Tensor, out: Optional[torch.Tensor]) -> Tuple:
+    """Checks a product's tensors: vectors, elements from vector to vector and from result to result, type, the result's
+    shape, whether the vectors have to be copied."""
+    shape, k, n = x.shape, self.in_features, self.out_features
+    if x.dtype not in _FLOATS or x.device != self.device or len(shape) < 1 or shape[-1] != k:
+      raise ValueError(f"x must be a float [..., {k}] tensor on {self.device}, got {x.dtype} {tuple(shape)} on {x.device}")
+    vectors = x.numel() // k
+    side_by_side = k == 1 or x.stride(-1) == 1
+    as_rows = side_by_side and (vectors == 1 or (x.dim() == 2 and x.stride(0) >= k))
+    want = (*shape[:-1], n)
+    pitch = n
+    if out is not None:
+      if out.dim() == 2 and out.shape == want and (n == 1 or out.stride(1) == 1) and (vectors <= 1 or out.stride(0) >= n):
+        pitch = out.stride(0)
+      elif out.shape != want or not out.is_contiguous():
+        raise ValueError(f"out must be {want} with its rows side by side, got {tuple(out.shape)} {out.stride()}")
+      if out.dtype != x.dtype or out.device != self.device:
+        raise ValueError(f"out must be {x.dtype} on {self.device}, got {out.dtype} on {out.device}")
+    return (vectors, x.stride(0) if as_rows and vectors > 1 else k, pitch, abi.DTYPES[x.dtype], want,
+            not (as_rows or x.is_contiguous()))
