@@ -25,7 +25,8 @@ struct DeviceScope {
   hipError_t status;
   explicit DeviceScope(int device) {
     (void)hipGetDevice(&prev);
-    status = hipSetDevice(device);
+    status = prev == device ? hipSuccess : hipSetDevice(device);
+    if (prev == device) prev = -1;
   }
   ~DeviceScope() {
     if (prev >= 0) (void)hipSetDevice(prev);

@@ -148,9 +148,10 @@ struct AttendParams {
   uint32_t* flags;
   int64_t table_stride;
   taco_divisor page16;                                    // 16-token blocks of a page
-  float* partial;                                    // the workgroups' partial results, see Partials
+  char* workspace;                                   // see Partials
   float scale_log2;                                  // scale * log2(e)
   int32_t n_seqs, table_width, n_pages, n_heads, n_q_heads, group, q_tiles, head_dim, window;
+  taco_divisor workgroups;                           // of the grid
   int32_t least;                                     // tiles of a workgroup's share at least
 };
 
@@ -377,11 +378,22 @@ struct Attend {
 // a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
 // by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
 // kernel joins in the order of the workgroups.
-// Divisions whose operands nearly always fit 32 bits (an operand that does not is an utterance line of 2^32 tiles).
-__device__ __forceinline__ uint64_t div64(uint64_t n, uint64_t d) {
-  return (n >> 32) || (d >> 32) ? n / d : (uint64_t)((uint32_t)n / (uint32_t)d);
-}
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
+
+// Inclusive sum over the lanes of a wave (DPP: shifts within rows of 16, then each row's last value to the next one's lanes,
+// then that of the lower half to the upper).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = add_dpp<0x111, 0xf>(v);      // row_shr:1, 2, 4, 8
+  v = add_dpp<0x112, 0xf>(v);
+  v = add_dpp<0x114, 0xf>(v);
+  v = add_dpp<0x118, 0xf>(v);
+  v = add_dpp<0x142, 0xa>(v);      // row_bcast:15
+  return add_dpp<0x143, 0xc>(v);   // row_bcast:31
+}
 
 // 64 utterances, one per lane: what each sees and how many tiles its rows have.
 template <int TT>
@@ -406,12 +418,7 @@ struct Utterances {
       low = a.window > 0 ? max(0, len - a.window) : 0;
       tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
     }
-    scan = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t u = __shfl_up(scan, d, 64);
-      if ((int)(threadIdx.x & 63) >= d) scan += u;
-    }
+    scan = wave_scan(tiles);
   }
   // Loads the first 64 and sums the tiles of all.
   __device__ __forceinline__ uint32_t load_all(const AttendParams& a, bool flag) {
@@ -431,25 +438,29 @@ struct Utterances {
       load(a, base + 64, false);
     }
   }
-  // Moves on to the 64 in which tile `at` lies (one row per utterance counted) and returns its utterance.
-  __device__ __forceinline__ int find(const AttendParams& a, uint32_t at) {
-    while (at - before >= lane_of(scan, 63)) move_to(a, base + 64);
-    return base + __popcll(__ballot(before + scan <= at));      // those that end at or before it
+  // Moves on to the 64 in which tile `at` of the line lies and returns its utterance.
+  __device__ __forceinline__ int find(const AttendParams& a, uint64_t at, uint32_t rows_per) {
+    while (at >= (uint64_t)(before + lane_of(scan, 63)) * rows_per) move_to(a, base + 64);
+    return base + __popcll(__ballot((uint64_t)(before + scan) * rows_per <= at));      // those that end at or before it
   }
   __device__ __forceinline__ uint32_t before_of(int b) const { return before + lane_of(scan, b - base) - lane_of(tiles, b - base); }
 };
 
-__device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all, uint32_t workgroups) {
-  const uint64_t share = div64(all + workgroups - 1, workgroups);
+// Tiles of a share (the division by the number of workgroups is a multiplication as long as it fits, see taco_divisor).
+__device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all) {
+  const uint64_t n = all + a.workgroups.div - 1;
+  const uint64_t share = n < (1u << 30) ? taco_divide((uint32_t)n, a.workgroups) : n / a.workgroups.div;
   return share < (uint64_t)a.least ? (uint64_t)a.least : share;
 }
+__device__ __forceinline__ uint64_t div64(uint64_t n, uint64_t d) { return (n | d) >> 32 ? n / d : (uint64_t)((uint32_t)n / (uint32_t)d); }
 
-// Partial results: first the maxima and sums of all of them, [2 per workgroup][queries][2], then the outputs [..][DP].
-template <int DP>
+// The workspace: for every row its first workgroup and how many it has, then the partial results' maxima and sums, [2 per
+// workgroup][queries][2], then their outputs [2 per workgroup][queries][DP].
 struct Partials {
+  taco_u2* rows;
   float *ml, *o;
-  __device__ __forceinline__ Partials(const AttendParams& a, uint32_t workgroups, int held)
-      : ml(a.partial), o(a.partial + (((size_t)workgroups * held * 4 + 3) & ~(size_t)3)) {}
+  __device__ __forceinline__ Partials(const AttendParams& a, uint32_t rows_per, int held)
+      : rows((taco_u2*)a.workspace), ml((float*)(rows + (((size_t)a.n_seqs * rows_per + 1) & ~(size_t)1))), o(ml + (size_t)a.workgroups.div * held * 4) {}
 };
 
 template <int T>
@@ -476,11 +487,11 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
   Utterances<A::TT> us;
-  const uint64_t all = (uint64_t)us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64) * rows_per, share = share_of(a, all, gridDim.x);
+  const uint64_t all = (uint64_t)us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64) * rows_per, share = share_of(a, all);
   uint64_t at = share * blockIdx.x;
   const uint64_t end = at + share < all ? at + share : all;
   if (at >= end) return;
-  int b = us.find(a, (uint32_t)div64(at, rows_per));
+  int b = us.find(a, at, rows_per);
   const int held = a.group < 16 ? a.group : 16;            // queries of a row in LDS and in the partial results
   bool first = true;
   uint64_t in = at - (uint64_t)us.before_of(b) * rows_per;     // tile within the utterance
@@ -490,7 +501,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     const uint32_t tiles = lane_of(us.tiles, b - us.base);
     const uint32_t row = (uint32_t)div64(in, tiles), tile0 = (uint32_t)(in - (uint64_t)row * tiles);
     const uint32_t n = (uint32_t)(end - at < tiles - tile0 ? end - at : tiles - tile0);
-    const int qt = row % a.q_tiles, h = row / a.q_tiles;
+    const int h = a.q_tiles == 1 ? row : row / a.q_tiles, qt = row - h * a.q_tiles;
     taco_u4 q[A::NQ];
     A::load_q(a, b, h, qt, q);
     float factor = a.scale_log2;
@@ -520,7 +531,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     __syncthreads();
     const int rows = min(a.group - qt * 16, 16);
     // a row that began in an earlier share is this workgroup's first partial result, one that only ends later its second
-    const Partials<DP> parts(a, gridDim.x, held);
+    const Partials parts(a, rows_per, held);
+    if (tile0 == 0 && threadIdx.x == 0)      // of how many shares the row is, the next ones holding `share` tiles each
+      parts.rows[(size_t)b * rows_per + row] = taco_u2{blockIdx.x, n == tiles ? 1 : 1 + (uint32_t)div64(tiles - n + share - 1, share)};
     const size_t slot = (size_t)(2 * blockIdx.x + (tile0 ? 0 : 1)) * held;
     for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
       const int r = i / DP, d = i % DP;
@@ -548,29 +561,25 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
   }
 }
 
-// Joins the rows that cross a border of shares: one workgroup per row and query, `workgroups` is the first kernel's grid.  A
-// long utterance alone leaves a hundred parts of a row, so the maxima are taken by 256 threads at a time and the outputs by as many
-// groups of DP / 4 threads as there are, each with its own parts, in a fixed order.
+// Joins the rows that cross a border of shares, one workgroup per row and query.  A long utterance alone leaves a hundred parts
+// of a row, so the maxima are taken by 256 threads at a time and the outputs by as many groups of DP / 4 threads as there are,
+// each with its own parts, in a fixed order.
 template <int T, int C, int DP>
-__global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a, uint32_t workgroups) {
-  using A = Attend<T, C, DP>;
+__global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a) {
   constexpr int GROUPS = 256 / (DP / 4);
   __shared__ float red[2][4], weight[256];
   __shared__ taco_f4 outs[GROUPS][DP / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t rows_per = a.n_heads * a.q_tiles;
-  const int held = a.group < 16 ? a.group : 16, r = blockIdx.x % held;
-  const uint32_t nth = blockIdx.x / held, row = nth % rows_per;
-  const int b = nth / rows_per, qt = row % a.q_tiles, h = row / a.q_tiles;
-  if (qt * 16 + r >= a.group) return;
-  Utterances<A::TT> us;
-  const uint64_t share = share_of(a, (uint64_t)us.load_all(a, false) * rows_per, workgroups);
-  us.move_to(a, b);
-  const uint32_t tiles = lane_of(us.tiles, b - us.base);
-  const uint64_t start = (uint64_t)us.before_of(b) * rows_per + (uint64_t)row * tiles, last = start + tiles - 1;
-  const uint32_t w0 = (uint32_t)div64(start, share), n = (uint32_t)div64(last, share) - w0 + 1;
+  const int held = a.group < 16 ? a.group : 16;
+  const Partials parts(a, rows_per, held);
+  const uint32_t nth = blockIdx.x / held;
+  const taco_u2 info = parts.rows[nth];
+  const uint32_t w0 = info[0], n = info[1];
   if (n == 1) return;
-  const Partials<DP> parts(a, workgroups, held);
+  const uint32_t row = nth % rows_per;
+  const int r = blockIdx.x % held, b = nth / rows_per, qt = row % a.q_tiles, h = row / a.q_tiles;
+  if (qt * 16 + r >= a.group) return;
   const auto at = [&](uint32_t k) { return (size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r; };
   float m = NEG_INF;
   for (uint32_t k = tid; k < n; k += 256) m = fmaxf(m, parts.ml[at(k) * 2]);
@@ -728,7 +737,7 @@ template <int T, int C, int DP>
 int launch_attend(const AttendParams& a, const Plan& p, hipStream_t s) {
   const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
   taco_kv_attend_kernel<T, C, DP><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
-  if (p.bytes) taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a, p.workgroups);
+  taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a);
   TACO_HIP(hipGetLastError());
   return TACO_OK;
 }
@@ -768,7 +777,7 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char
   p.least = AT_WAVES;
   const int64_t most = (rows * (tiles < 1 ? 1 : tiles) + p.least - 1) / p.least;
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
-  p.bytes = ((int64_t)p.workgroups * p.held * 4 + 3) / 4 * 16 + (int64_t)2 * p.workgroups * p.held * p.dp * 4;
+  p.bytes = (rows + 1) / 2 * 16 + (int64_t)2 * p.workgroups * p.held * (2 + p.dp) * 4;
   return TACO_OK;
 }
 
@@ -817,14 +826,15 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
   Plan p;
   rc = plan_attend(c, t, who, p);
   if (rc != TACO_OK) return rc;
-  if (p.bytes && (!t->workspace || !aligned(t->workspace) || t->workspace_bytes < p.bytes)) TACO_FAIL(TACO_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes, has %lld", who, (long long)p.bytes, (long long)t->workspace_bytes);
+  if ((!t->workspace || !aligned(t->workspace) || t->workspace_bytes < p.bytes)) TACO_FAIL(TACO_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes, has %lld", who, (long long)p.bytes, (long long)t->workspace_bytes);
   a.k_pages = (const char*)c->k; a.v_pages = (const char*)c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale;
   a.q = (const char*)t->q; a.out = (char*)t->out; a.lse = t->lse; a.table = t->table; a.lens = t->lens; a.flags = c->flags;
   a.table_stride = t->table_stride; a.page16 = taco_make_divisor((uint32_t)c->page_size / 16);
   a.scale_log2 = t->scale * 1.44269504088896340736f;
   a.n_seqs = t->n_seqs; a.table_width = t->table_width; a.n_pages = c->n_pages; a.n_heads = c->n_heads;
   a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.window = t->window;
-  a.group = p.group; a.q_tiles = p.q_tiles; a.partial = (float*)t->workspace; a.least = (int)p.least;
+  a.group = p.group; a.q_tiles = p.q_tiles; a.workspace = (char*)t->workspace; a.least = (int)p.least;
+  a.workgroups = taco_make_divisor(p.workgroups);
   return by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return launch_attend<ty.value, ca.value, dp.value>(a, p, (hipStream_t)stream); });
 }
 
