@@ -325,7 +325,8 @@ typedef struct taco_kv_attend_args {
 
 /* Attention of one new token per utterance: out = sum_t w_t v_t, w = softmax over the seen tokens of scale * (q . k_t);
  * query head h reads cache head h / (n_q_heads / n_heads).  lse gets the natural logarithm of the softmax's sum.  An
- * utterance without seen tokens (length 0, or none left by bad table entries, which set a flag) gets zeros and -inf.
+ * utterance without seen tokens (length 0, none left by bad table entries, which set a flag, no score above -inf) gets zeros
+ * and -inf.
  * Slots at and behind lens[b] may hold anything.  Statistics and sums are fp32; results do not depend on timing. */
 int taco_kv_attend(const taco_kv_cache* cache, const taco_kv_attend_args* args, void* stream);
 

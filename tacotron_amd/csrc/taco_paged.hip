@@ -152,10 +152,10 @@ struct AttendParams {
   float scale_log2;                                  // scale * log2(e)
   int32_t n_seqs, table_width, n_pages, n_heads, n_q_heads, group, q_tiles, head_dim, window;
   taco_divisor workgroups;                           // of the grid
-  int32_t least;                                     // tiles of a workgroup's share at least
 };
 
 constexpr int AT_WAVES = 4;
+constexpr uint32_t LEAST = AT_WAVES;       // tiles of a workgroup at least: one for every wave
 constexpr float NEG_INF = -__builtin_inff();
 
 // What a wave holds of one (utterance, cache head, up to 16 query heads): the running maximum and sum of the softmax of
@@ -377,7 +377,11 @@ struct Attend {
 // workgroup of a grid that fills the GPU once, whatever the lengths are: a long utterance alone is split over its length,
 // a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
 // by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
-// kernel joins in the order of the workgroups.
+// kernel joins in the order of the workgroups.  A workgroup whose share holds the end of one row and the beginning of the next
+// starts twice, 2 to 3 us each.  So where the tiles are so few that every row can be cut into parts of four tiles of its own, one
+// workgroup each, that is done instead (777 tokens of 8 heads of 128: 6 against 10 us).  Joining in the first kernel, by the last
+// workgroup of a row, was slower: what the others wrote has to be stored through to memory and awaited (sixteen lines 35
+// against 31 us, with a fence 211).
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 
 // Inclusive sum over the lanes of a wave (DPP: shifts within rows of 16, then each row's last value to the next one's lanes,
@@ -395,19 +399,24 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   return add_dpp<0x143, 0xc>(v);   // row_bcast:31
 }
 
+// What a sum over utterances counts, of one row each: tiles, and parts of LEAST tiles.
+struct Count {
+  uint32_t tiles, parts;
+};
+
 // 64 utterances, one per lane: what each sees and how many tiles its rows have.
 template <int TT>
 struct Utterances {
   int base;                  // the first of them
-  uint32_t before;           // tiles of one row of every utterance in front of them
+  Count before;              // of the utterances in front of them
   int low, len;              // seen tokens [low, len) of this lane's utterance
-  uint32_t tiles, scan;      // tiles of one of its rows (one that sees nothing has one, so that somebody writes its zeros); inclusive sum
+  Count own, scan;           // of its rows (one that sees nothing has a tile, so that somebody writes its zeros); inclusive sum
 
   __device__ __forceinline__ void load(const AttendParams& a, int first, bool flag) {
     base = first;
     const int b = first + (threadIdx.x & 63);
     len = low = 0;
-    tiles = 0;
+    own.tiles = 0;
     if (b < a.n_seqs) {
       len = a.lens[b];
       const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
@@ -416,41 +425,45 @@ struct Utterances {
         len = len < 0 ? 0 : (int)room;
       }
       low = a.window > 0 ? max(0, len - a.window) : 0;
-      tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
+      own.tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
     }
-    scan = wave_scan(tiles);
+    own.parts = (own.tiles + LEAST - 1) / LEAST;
+    scan = {wave_scan(own.tiles), wave_scan(own.parts)};
   }
-  // Loads the first 64 and sums the tiles of all.
-  __device__ __forceinline__ uint32_t load_all(const AttendParams& a, bool flag) {
-    uint32_t sum = 0;
+  __device__ __forceinline__ Count last() const { return {lane_of(scan.tiles, 63), lane_of(scan.parts, 63)}; }
+  // Loads the first 64 and counts all.
+  __device__ __forceinline__ Count load_all(const AttendParams& a, bool flag) {
+    Count sum = {0, 0};
     for (int i = 64; i < a.n_seqs; i += 64) {
       load(a, i, flag);
-      sum += lane_of(scan, 63);
+      sum = {sum.tiles + last().tiles, sum.parts + last().parts};
     }
     load(a, 0, flag);
-    before = 0;
-    return sum + lane_of(scan, 63);
+    before = {0, 0};
+    return {sum.tiles + last().tiles, sum.parts + last().parts};
   }
   // Moves on to the 64 that utterance `b` is one of.
   __device__ __forceinline__ void move_to(const AttendParams& a, int b) {
     while (b >= base + 64) {
-      before += lane_of(scan, 63);
+      before = {before.tiles + last().tiles, before.parts + last().parts};
       load(a, base + 64, false);
     }
   }
-  // Moves on to the 64 in which tile `at` of the line lies and returns its utterance.
-  __device__ __forceinline__ int find(const AttendParams& a, uint64_t at, uint32_t rows_per) {
-    while (at >= (uint64_t)(before + lane_of(scan, 63)) * rows_per) move_to(a, base + 64);
-    return base + __popcll(__ballot((uint64_t)(before + scan) * rows_per <= at));      // those that end at or before it
+  // Moves on to the 64 in which unit `at` of all rows lies (N: the unit) and returns its utterance; `at` becomes the unit within it.
+  template <uint32_t Count::*N>
+  __device__ __forceinline__ int find(const AttendParams& a, uint64_t& at, uint32_t rows_per) {
+    while (at >= (uint64_t)(before.*N + lane_of(scan.*N, 63)) * rows_per) move_to(a, base + 64);
+    const int lane = __popcll(__ballot((uint64_t)(before.*N + scan.*N) * rows_per <= at));      // those that end at or before it
+    at -= (uint64_t)(before.*N + lane_of(scan.*N, lane) - lane_of(own.*N, lane)) * rows_per;
+    return base + lane;
   }
-  __device__ __forceinline__ uint32_t before_of(int b) const { return before + lane_of(scan, b - base) - lane_of(tiles, b - base); }
 };
 
 // Tiles of a share (the division by the number of workgroups is a multiplication as long as it fits, see taco_divisor).
 __device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all) {
   const uint64_t n = all + a.workgroups.div - 1;
   const uint64_t share = n < (1u << 30) ? taco_divide((uint32_t)n, a.workgroups) : n / a.workgroups.div;
-  return share < (uint64_t)a.least ? (uint64_t)a.least : share;
+  return share < LEAST ? LEAST : share;
 }
 __device__ __forceinline__ uint64_t div64(uint64_t n, uint64_t d) { return (n | d) >> 32 ? n / d : (uint64_t)((uint32_t)n / (uint32_t)d); }
 
@@ -487,20 +500,39 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
   Utterances<A::TT> us;
-  const uint64_t all = (uint64_t)us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64) * rows_per, share = share_of(a, all);
-  uint64_t at = share * blockIdx.x;
-  const uint64_t end = at + share < all ? at + share : all;
-  if (at >= end) return;
-  int b = us.find(a, at, rows_per);
+  const Count count = us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64);
+  uint64_t at, share, left;               // where this workgroup begins, how many tiles it takes
+  uint32_t row, tile0;
+  int b;
+  const uint64_t all_parts = (uint64_t)count.parts * rows_per;
+  const bool apart = all_parts <= gridDim.x;      // every row on its own
+  if (apart) {
+    at = blockIdx.x;
+    if (at >= all_parts) return;
+    b = us.template find<&Count::parts>(a, at, rows_per);
+    const uint32_t parts = lane_of(us.own.parts, b - us.base), tiles = lane_of(us.own.tiles, b - us.base);
+    share = (tiles + parts - 1) / parts;
+    row = (uint32_t)at / parts;
+    tile0 = ((uint32_t)at - row * parts) * (uint32_t)share;
+    if (tile0 >= tiles) return;           // an even cut may need fewer parts
+    left = min((uint32_t)share, tiles - tile0);
+  } else {
+    const uint64_t all = (uint64_t)count.tiles * rows_per;
+    share = share_of(a, all);
+    at = share * blockIdx.x;
+    if (at >= all) return;
+    left = min(share, all - at);
+    b = us.template find<&Count::tiles>(a, at, rows_per);
+    const uint32_t tiles = lane_of(us.own.tiles, b - us.base);
+    row = (uint32_t)div64(at, tiles);
+    tile0 = (uint32_t)(at - (uint64_t)row * tiles);
+  }
   const int held = a.group < 16 ? a.group : 16;            // queries of a row in LDS and in the partial results
-  bool first = true;
-  uint64_t in = at - (uint64_t)us.before_of(b) * rows_per;     // tile within the utterance
-  while (at < end) {
+  for (bool first = true; left; first = false) {
     us.move_to(a, b);
     const int low = (int)lane_of(us.low, b - us.base), len = (int)lane_of(us.len, b - us.base);
-    const uint32_t tiles = lane_of(us.tiles, b - us.base);
-    const uint32_t row = (uint32_t)div64(in, tiles), tile0 = (uint32_t)(in - (uint64_t)row * tiles);
-    const uint32_t n = (uint32_t)(end - at < tiles - tile0 ? end - at : tiles - tile0);
+    const uint32_t tiles = lane_of(us.own.tiles, b - us.base);
+    const uint32_t n = left < tiles - tile0 ? (uint32_t)left : tiles - tile0;
     const int h = a.q_tiles == 1 ? row : row / a.q_tiles, qt = row - h * a.q_tiles;
     taco_u4 q[A::NQ];
     A::load_q(a, b, h, qt, q);
@@ -516,7 +548,6 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
       for (uint32_t t = wave; t < n; t += AT_WAVES) A::tile(a, b, h, base + (int)t * A::TT, low, len, factor, q, st);
     // join the waves: [wave][query][m, l, DP outputs]
     if (!first) __syncthreads();
-    first = false;
     const float l = taco_sum_rows(st.l);
     if (col < held) {
       float* mine = lds + (wave * held + col) * (DP + 2);
@@ -555,9 +586,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
         parts.o[(slot + r) * DP + d] = o;
       }
     }
-    at += n;
-    in += n;
-    if (in == (uint64_t)tiles * rows_per) { in = 0; ++b; }
+    left -= n;
+    tile0 = 0;
+    if (++row == rows_per) { row = 0; ++b; }
   }
 }
 
@@ -712,7 +743,7 @@ namespace {
 // Everything about a call that its sizes decide.
 struct Plan {
   int group, q_tiles, held, dp, tt;
-  uint32_t workgroups, least;
+  uint32_t workgroups;
   int64_t bytes;
 };
 
@@ -773,9 +804,8 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char
   if (rc != TACO_OK) return rc;
   const int64_t rows = (int64_t)t->n_seqs * c->n_heads * p.q_tiles;
   const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
-  // a share has a tile for every wave at least; no more workgroups than that leaves work for
-  p.least = AT_WAVES;
-  const int64_t most = (rows * (tiles < 1 ? 1 : tiles) + p.least - 1) / p.least;
+  // no more workgroups than there are parts when every row is cut on its own
+  const int64_t most = rows * (((tiles < 1 ? 1 : tiles) + LEAST - 1) / LEAST);
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
   p.bytes = (rows + 1) / 2 * 16 + (int64_t)2 * p.workgroups * p.held * (2 + p.dp) * 4;
   return TACO_OK;
@@ -833,7 +863,7 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
   a.scale_log2 = t->scale * 1.44269504088896340736f;
   a.n_seqs = t->n_seqs; a.table_width = t->table_width; a.n_pages = c->n_pages; a.n_heads = c->n_heads;
   a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.window = t->window;
-  a.group = p.group; a.q_tiles = p.q_tiles; a.workspace = (char*)t->workspace; a.least = (int)p.least;
+  a.group = p.group; a.q_tiles = p.q_tiles; a.workspace = (char*)t->workspace;
   a.workgroups = taco_make_divisor(p.workgroups);
   return by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return launch_attend<ty.value, ca.value, dp.value>(a, p, (hipStream_t)stream); });
 }
