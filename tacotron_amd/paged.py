@@ -45,6 +45,16 @@ def _rows_ok(t: torch.Tensor) -> bool:
   return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s * size % 16 == 0 for s in t.stride()[:-1])
 
 
+def _apart(t: torch.Tensor) -> bool:
+  """Whether no two elements of ``t`` share an address."""
+  extent = 1
+  for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
+    if stride < extent:
+      return False
+    extent = stride * (size - 1) + extent
+  return True
+
+
 class PagedCache:
   """``n_pages`` pages of ``page_size`` tokens of ``n_heads`` heads of ``head_dim`` elements, keys and values.
 
@@ -86,8 +96,8 @@ class PagedCache:
       raise ValueError(f"page_size {page_size} and head_dim {head_dim} must be multiples of 16, head_dim at most 256, and "
                        f"neither pages ({n_pages}) nor heads ({n_heads}) may be missing")
     self.device = _device(k.device)
-    if not (_rows_ok(k) and _rows_ok(v)):
-      raise ValueError("rows of the cache must have unit stride and start at multiples of 16 bytes")
+    if not (_rows_ok(k) and _rows_ok(v) and _apart(k) and _apart(v)):
+      raise ValueError("rows of the cache must have unit stride, start at multiples of 16 bytes and not overlap")
     if k.dtype == torch.float8_e4m3fn:
       k_scale, v_scale = (torch.ones(n_heads, device=self.device) if s is None else s for s in (k_scale, v_scale))
       _check_vector(k_scale, "k_scale", torch.float32, n_heads, self.device)
@@ -106,7 +116,7 @@ class PagedCache:
     self._lib = _lib.lib()
     # what a call's checks have found, by the shapes, strides, types and devices of its tensors (never by their addresses)
     self._append_forms: Dict[Tuple, bytes] = {}
-    self._attend_forms: Dict[Tuple, Tuple[bytes, int]] = {}
+    self._attend_forms: Dict[Tuple, Tuple[bytes, int, torch.Tensor]] = {}
 
   @property
   def n_pages(self) -> int:
@@ -132,9 +142,9 @@ class PagedCache:
       raise ValueError(f"{name} must be {' or '.join(str(d) for d in self._takes)} on {self.device}, got {t.dtype} on {t.device}")
 
   def _out(self, out: torch.Tensor, like: torch.Tensor) -> None:
-    if out.shape != like.shape or out.dtype != like.dtype or out.device != self.device or not _rows_ok(out):
-      raise ValueError(f"out must be {like.dtype} {tuple(like.shape)} on {self.device} with unit stride and rows at multiples of "
-                       f"16 bytes, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != self.device or not _rows_ok(out) or not _apart(out):
+      raise ValueError(f"out must be {like.dtype} {tuple(like.shape)} on {self.device} with unit stride and separate rows at "
+                       f"multiples of 16 bytes, got {out.dtype} {tuple(out.shape)} on {out.device}")
 
   def _index(self, t: torch.Tensor, name: str, size: int) -> None:
     if t.dtype != torch.int32 or t.shape != (size,) or t.device != self.device or not t.is_contiguous():
@@ -174,7 +184,7 @@ class PagedCache:
       k, v = rows[0], rows[1]      # kept until the call is enqueued
       kp, vp, qp = k.data_ptr(), v.data_ptr(), 0 if q is None else rows[2].data_ptr()
     if q is not None and out is None:
-      out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+      out = _lib.new(q)
       op = out.data_ptr()
     if kp:      # no tokens have no address
       head = _APPEND_POINTERS.pack(kp, vp, qp, op, table.data_ptr(), past.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
@@ -237,11 +247,11 @@ class PagedCache:
         self._attend_forms[key] = found
       q = rows      # kept until the call is enqueued
       qp = q.data_ptr()
-    tail, need = found
+    tail, need, lse_form = found
     if out is None:
-      out = torch.empty(q.shape, dtype=q.dtype, device=self.device)
+      out = _lib.new(q)
       op = out.data_ptr()
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
+    lse = _lib.new(lse_form) if return_lse else None
     if op:        # no utterances have no address
       # allocated per call: the allocator orders its reuse by stream, and a captured graph gets one of its own
       work = torch.empty(need, dtype=torch.uint8, device=self.device)
@@ -251,8 +261,9 @@ class PagedCache:
         _lib.check(rc)
     return (out, lse) if return_lse else out
 
-  def _attend_tail(self, q, table, lens, scale, window, out) -> Tuple[bytes, int]:
-    """Checks an attend's tensors; the part of its argument block that their forms decide, and its workspace."""
+  def _attend_tail(self, q, table, lens, scale, window, out) -> Tuple[bytes, int, torch.Tensor]:
+    """Checks an attend's tensors; the part of its argument block that their forms decide, the size of its workspace, the form
+    of its logarithms."""
     n, width = self._table(table)
     self._rows(q, "q", n, None)
     heads = q.shape[1]
@@ -271,7 +282,7 @@ class PagedCache:
     if need < 0:
       _lib.check(int(need))
     a.workspace_bytes = need
-    return bytes(a)[_ATTEND_POINTERS.size:], need
+    return bytes(a)[_ATTEND_POINTERS.size:], need, _lib.shape_of((n, heads), torch.float32, self.device)
 
   def check(self) -> None:
     """Waits for the current stream and raises an IndexError if a call since the last check has met a table entry that is

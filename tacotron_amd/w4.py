@@ -135,7 +135,7 @@ class W4Matrix:
     if copies:        # columns apart, expanded or overlapping vectors
       x = x.contiguous()
     if out is None:
-      out = torch.empty(want, dtype=x.dtype, device=self.device)
+      out = _lib.new(want)
     if n:
       rc = self._lib.taco_qmat_multiply(self._ref, x.data_ptr(), x_pitch, out.data_ptr(), y_pitch, n, code,
                                         _lib.raw_stream(self._c.device))
@@ -145,7 +145,7 @@ class W4Matrix:
 
   def _form(self, x: torch.Tensor, out: Optional[torch.Tensor]) -> Tuple:
     """Checks a product's tensors: vectors, elements from vector to vector and from result to result, type, the result's
-    shape, whether the vectors have to be copied."""
+    form, whether the vectors have to be copied."""
     shape, k, n = x.shape, self.in_features, self.out_features
     if x.dtype not in _FLOATS or x.device != self.device or len(shape) < 1 or shape[-1] != k:
       raise ValueError(f"x must be a float [..., {k}] tensor on {self.device}, got {x.dtype} {tuple(shape)} on {x.device}")
@@ -161,5 +161,5 @@ class W4Matrix:
         raise ValueError(f"out must be {want} with its rows side by side, got {tuple(out.shape)} {out.stride()}")
       if out.dtype != x.dtype or out.device != self.device:
         raise ValueError(f"out must be {x.dtype} on {self.device}, got {out.dtype} on {out.device}")
-    return (vectors, x.stride(0) if as_rows and vectors > 1 else k, pitch, abi.DTYPES[x.dtype], want,
-            not (as_rows or x.is_contiguous()))
+    return (vectors, x.stride(0) if as_rows and vectors > 1 else k, pitch, abi.DTYPES[x.dtype],
+            _lib.shape_of(want, x.dtype, self.device), not (as_rows or x.is_contiguous()))

@@ -429,7 +429,10 @@ def test_refused_tensors():
     lambda: cache.append(k, k, i(2, 3).t(), i(3)), lambda: cache.append(k.cpu(), k.cpu(), i(3, 2), i(3)),
     lambda: cache.attend(t(3, 3, 64), i(3, 2), i(3)), lambda: cache.attend(t(3, 4, 32), i(3, 2), i(3)), lambda: cache.attend(t(3, 4, 64), i(2, 2), i(2)),
     lambda: cache.attend(t(3, 4, 64), i(3, 2), i(3), window=-1), lambda: cache.attend(t(3, 4, 64, dtype=F16), i(3, 2), i(3)),
-    lambda: cache.attend(t(3, 4, 64), i(3, 2), i(3), out=t(3, 4, 66)[..., 2:]), lambda: cache.attend(t(3, 4, 64), i(3, 2).cpu(), i(3)),
+    lambda: cache.attend(t(3, 4, 64), i(3, 2), i(3), out=t(3, 4, 66)[..., 2:]),
+    lambda: cache.attend(t(3, 4, 64), i(3, 2), i(3), out=t(3, 1, 64).expand(3, 4, 64)),
+    lambda: cache.append(k, k, i(3, 2), i(3), q=k, out=t(1, 2, 64).expand(3, 2, 64)),
+    lambda: PagedCache.from_tensors(t(1, 16, 2, 64).expand(4, 16, 2, 64), t(4, 16, 2, 64)), lambda: cache.attend(t(3, 4, 64), i(3, 2).cpu(), i(3)),
   ):
     with pytest.raises((ValueError, RuntimeError)):
       call()
