@@ -176,7 +176,11 @@ struct State {
 //     them is one operand: for 16-bit types a v_perm per word turns rows into operands.
 // Weights are rounded to the operand type twice, p = hi + lo: one rounding alone would be as large as that of the
 // output itself, and the second product costs nothing while memory is the bound.
-template <int T, int C, int DP>
+// K and V serve 16 * QT query heads of a cache head; further ones read them again.  With more than 16, QT = 2 pays where reading
+// is the bound (16 x 16384 tokens, 2 heads of 128 in bfloat16, 64 query heads: 82 us with QT = 1, 71 with 2; 16 x 60000 tokens
+// of 64 elements, 64 query heads over one: 144 and 90), not for fp32, whose products are slower than its reading (48 query
+// heads over 2 of 128: 78 and 86).
+template <int T, int C, int DP, int QT>
 struct Attend {
   static constexpr int CB = taco_size_of<C>;
   static constexpr int TT = C == TACO_F32 ? 16 : 32;           // tokens of a tile
@@ -190,22 +194,27 @@ struct Attend {
   using St = State<NB, VE>;
 
   // Query operands: for the K operand whose lane holds elements d0 .. of a row, the same elements of query column l & 15.
-  static __device__ void load_q(const AttendParams& a, int b, int h, int qt, taco_u4 (&q)[NQ]) {
+  using Queries = taco_u4[QT][NQ];
+  static __device__ void load_q(const AttendParams& a, int b, int h, int qt, Queries& q) {
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    const bool have = qt * 16 + col < a.group;
-    const char* row = a.q + (int64_t)b * a.q_st[0] + (int64_t)(h * a.group + qt * 16 + (have ? col : 0)) * a.q_st[1];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      int d;      // first element
-      if constexpr (C == TACO_E4M3) d = (n >> 1) * 64 + g * 16 + (n & 1) * 8;
-      else d = (n * 4 + g) * KE;
-      q[n] = taco_u4{0, 0, 0, 0};
-      if (have && d < a.head_dim) q[n] = *(const taco_u4*)(row + (int64_t)d * taco_size_of<T>);
+    for (int t = 0; t < QT; ++t) {
+      const int nth = (qt * QT + t) * 16 + col;
+      const bool have = nth < a.group;
+      const char* row = a.q + (int64_t)b * a.q_st[0] + (int64_t)(h * a.group + (have ? nth : 0)) * a.q_st[1];
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        int d;      // first element
+        if constexpr (C == TACO_E4M3) d = (n >> 1) * 64 + g * 16 + (n & 1) * 8;
+        else d = (n * 4 + g) * KE;
+        q[t][n] = taco_u4{0, 0, 0, 0};
+        if (have && d < a.head_dim) q[t][n] = *(const taco_u4*)(row + (int64_t)d * taco_size_of<T>);
+      }
     }
   }
 
   static __device__ __forceinline__ void tile(const AttendParams& a, int b, int h, int t0, int low, int len, float factor,
-                                              const taco_u4 (&q)[NQ], St& st) {
+                                              const Queries& q, St (&st)[QT]) {
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     // the pages of the tile's 16-token blocks; a block behind the last token, or on a bad page, reads page 0 and is masked
     const int32_t* row = a.table + (int64_t)b * a.table_stride;
@@ -260,28 +269,36 @@ struct Attend {
         }
       }
     // scores
-    float p[SUB * 4];
+    float p[QT][SUB * 4];
 #pragma unroll
     for (int s = 0; s < SUB; ++s) {
-      taco_f4 acc = {0, 0, 0, 0};
+      taco_f4 acc[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) acc[t] = taco_f4{0, 0, 0, 0};
 #pragma unroll
       for (int n = 0; n < NK; ++n) {
         if constexpr (C == TACO_F32) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[s][n][e]), __uint_as_float(q[n][e]), acc, 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[s][n][e]), __uint_as_float(q[t][n][e]), acc[t], 0, 0, 0);
         } else if constexpr (C == TACO_E4M3) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const taco_u4 x = {widen<0>(kr[s][n][2 * e]), widen<1>(kr[s][n][2 * e]), widen<0>(kr[s][n][2 * e + 1]), widen<1>(kr[s][n][2 * e + 1])};
-            acc = taco_mfma32<T>(x, q[2 * n + e], acc);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) acc[t] = taco_mfma32<T>(x, q[t][2 * n + e], acc[t]);
           }
         } else {
-          acc = taco_mfma32<T>(kr[s][n], q[n], acc);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) acc[t] = taco_mfma32<T>(kr[s][n], q[t][n], acc[t]);
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[s * 4 + i] = acc[i] * factor;
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[t][s * 4 + i] = acc[t][i] * factor;
     }
     // masked tokens: their weight is 0, and what lies in their V rows must not meet it (0 * NaN)
     bool whole = t0 >= low && t0 + TT <= len;
@@ -292,9 +309,10 @@ struct Attend {
       for (int s = 0; s < SUB; ++s)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int t = t0 + s * 16 + g * 4 + i;
-          if (!(ok[s] && t >= low && t < len)) {
-            p[s * 4 + i] = NEG_INF;
+          const int at = t0 + s * 16 + g * 4 + i;
+          if (!(ok[s] && at >= low && at < len)) {
+#pragma unroll
+            for (int t = 0; t < QT; ++t) p[t][s * 4 + i] = NEG_INF;
 #pragma unroll
             for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
@@ -303,25 +321,38 @@ struct Attend {
         }
     }
     // running maximum; the outputs are rescaled only in the tiles that raise it
-    float top = p[0];
+    taco_u4 hi[QT], lo[QT];
 #pragma unroll
-    for (int i = 1; i < SUB * 4; ++i) top = fmaxf(top, p[i]);
-    top = taco_max_rows(top);
-    if (__any(top > st.m)) {
-      const float m = fmaxf(st.m, top);
-      const float f = m == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(st.m - m);
-      st.m = m;
-      st.l *= f;
+    for (int t = 0; t < QT; ++t) {
+      St& own = st[t];
+      float top = p[t][0];
 #pragma unroll
-      for (int blk = 0; blk < NB; ++blk)
+      for (int i = 1; i < SUB * 4; ++i) top = fmaxf(top, p[t][i]);
+      top = taco_max_rows(top);
+      if (__any(top > own.m)) {
+        const float m = fmaxf(own.m, top);
+        const float f = m == NEG_INF ? 1.0f : __builtin_amdgcn_exp2f(own.m - m);
+        own.m = m;
+        own.l *= f;
 #pragma unroll
-        for (int e = 0; e < VE; ++e) st.o[blk][e] *= f;
-    }
-    const float m = st.m == NEG_INF ? 0.0f : st.m;
+        for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
-    for (int i = 0; i < SUB * 4; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(p[i] - m);
-      st.l += p[i];
+          for (int e = 0; e < VE; ++e) own.o[blk][e] *= f;
+      }
+      const float m = own.m == NEG_INF ? 0.0f : own.m;
+#pragma unroll
+      for (int i = 0; i < SUB * 4; ++i) {
+        p[t][i] = __builtin_amdgcn_exp2f(p[t][i] - m);
+        own.l += p[t][i];
+      }
+      if constexpr (C != TACO_F32) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          hi[t][w] = taco_pack2<T>(p[t][2 * w], p[t][2 * w + 1]);
+          const uint32_t both = hi[t][w];
+          lo[t][w] = taco_pack2<T>(p[t][2 * w] - taco_low<T>(both), p[t][2 * w + 1] - taco_high<T>(both));
+        }
+      }
     }
     // output
     if constexpr (C == TACO_F32) {
@@ -331,14 +362,10 @@ struct Attend {
         for (int e = 0; e < VE; ++e)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            st.o[blk][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][blk][e]), p[i], st.o[blk][e], 0, 0, 0);
-    } else {
-      taco_u4 hi, lo;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        hi[w] = taco_pack2<T>(p[2 * w], p[2 * w + 1]);
-        lo[w] = taco_pack2<T>(p[2 * w] - taco_low<T>(hi[w]), p[2 * w + 1] - taco_high<T>(hi[w]));
-      }
+            for (int t = 0; t < QT; ++t)
+              st[t].o[blk][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[i][blk][e]), p[t][i], st[t].o[blk][e], 0, 0, 0);
+    } else {
 #pragma unroll
       for (int blk = 0; blk < NB; ++blk)
 #pragma unroll
@@ -355,10 +382,14 @@ struct Attend {
             even[t] = __builtin_amdgcn_perm(x[2 * t + 1], x[2 * t], 0x05040100u);
             odd[t] = __builtin_amdgcn_perm(x[2 * t + 1], x[2 * t], 0x07060302u);
           }
-          st.o[blk][2 * w] = taco_mfma32<T>(even, hi, st.o[blk][2 * w]);
-          st.o[blk][2 * w] = taco_mfma32<T>(even, lo, st.o[blk][2 * w]);
-          st.o[blk][2 * w + 1] = taco_mfma32<T>(odd, hi, st.o[blk][2 * w + 1]);
-          st.o[blk][2 * w + 1] = taco_mfma32<T>(odd, lo, st.o[blk][2 * w + 1]);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) {
+            taco_f4 &o0 = st[t].o[blk][2 * w], &o1 = st[t].o[blk][2 * w + 1];
+            o0 = taco_mfma32<T>(even, hi[t], o0);
+            o1 = taco_mfma32<T>(odd, hi[t], o1);
+            o0 = taco_mfma32<T>(even, lo[t], o0);
+            o1 = taco_mfma32<T>(odd, lo[t], o1);
+          }
         }
     }
   }
@@ -372,8 +403,8 @@ struct Attend {
 };
 
 // ---- who does what ----
-// All tiles of a call stand in one line: utterance by utterance, within it row by row (a row: one cache head and up to 16 of
-// its query heads), within a row from the first seen tile to the last.  The line is cut into equal shares, one per
+// All tiles of a call stand in one line: utterance by utterance, within it row by row (a row: one cache head and up to 16 or
+// 32 of its query heads), within a row from the first seen tile to the last.  The line is cut into equal shares, one per
 // workgroup of a grid that fills the GPU once, whatever the lengths are: a long utterance alone is split over its length,
 // a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
 // by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
@@ -493,9 +524,9 @@ __device__ __forceinline__ void finish(const AttendParams& a, int b, int head, i
 // What a part counts for beside the common maximum.
 __device__ __forceinline__ float weight_of(float m_part, float m) { return m_part == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_part - m); }
 
-template <int T, int C, int DP>
+template <int T, int C, int DP, int QT>
 __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const AttendParams a) {
-  using A = Attend<T, C, DP>;
+  using A = Attend<T, C, DP, QT>;
   extern __shared__ float lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
@@ -527,40 +558,45 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     row = (uint32_t)div64(at, tiles);
     tile0 = (uint32_t)(at - (uint64_t)row * tiles);
   }
-  const int held = a.group < 16 ? a.group : 16;            // queries of a row in LDS and in the partial results
+  const int held = min(a.group, 16 * QT);            // queries of a row in LDS and in the partial results
   for (bool first = true; left; first = false) {
     us.move_to(a, b);
     const int low = (int)lane_of(us.low, b - us.base), len = (int)lane_of(us.len, b - us.base);
     const uint32_t tiles = lane_of(us.own.tiles, b - us.base);
     const uint32_t n = left < tiles - tile0 ? (uint32_t)left : tiles - tile0;
     const int h = a.q_tiles == 1 ? row : row / a.q_tiles, qt = row - h * a.q_tiles;
-    taco_u4 q[A::NQ];
+    typename A::Queries q;
     A::load_q(a, b, h, qt, q);
     float factor = a.scale_log2;
     if (C == TACO_E4M3) factor *= a.k_scale[h];
-    typename A::St st;
+    typename A::St st[QT];
 #pragma unroll
-    for (int blk = 0; blk < A::NB; ++blk)
+    for (int t = 0; t < QT; ++t)
 #pragma unroll
-      for (int e = 0; e < A::VE; ++e) st.o[blk][e] = taco_f4{0, 0, 0, 0};
+      for (int blk = 0; blk < A::NB; ++blk)
+#pragma unroll
+        for (int e = 0; e < A::VE; ++e) st[t].o[blk][e] = taco_f4{0, 0, 0, 0};
     const int base = (low / A::TT + (int)tile0) * A::TT;
     if (len > low)
       for (uint32_t t = wave; t < n; t += AT_WAVES) A::tile(a, b, h, base + (int)t * A::TT, low, len, factor, q, st);
     // join the waves: [wave][query][m, l, DP outputs]
     if (!first) __syncthreads();
-    const float l = taco_sum_rows(st.l);
-    if (col < held) {
-      float* mine = lds + (wave * held + col) * (DP + 2);
-      if (g == 0) { mine[0] = st.m; mine[1] = l; }
 #pragma unroll
-      for (int blk = 0; blk < A::NB; ++blk)
+    for (int t = 0; t < QT; ++t) {
+      const float l = taco_sum_rows(st[t].l);
+      if (t * 16 + col < held) {
+        float* mine = lds + (wave * held + t * 16 + col) * (DP + 2);
+        if (g == 0) { mine[0] = st[t].m; mine[1] = l; }
 #pragma unroll
-        for (int e = 0; e < A::VE; ++e)
+        for (int blk = 0; blk < A::NB; ++blk)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mine[2 + blk * 16 * A::VE + (4 * g + i) * A::VE + e] = st.o[blk][e][i];
+          for (int e = 0; e < A::VE; ++e)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[2 + blk * 16 * A::VE + (4 * g + i) * A::VE + e] = st[t].o[blk][e][i];
+      }
     }
     __syncthreads();
-    const int rows = min(a.group - qt * 16, 16);
+    const int rows = min(a.group - qt * 16 * QT, 16 * QT);
     // a row that began in an earlier share is this workgroup's first partial result, one that only ends later its second
     const Partials parts(a, rows_per, held);
     if (tile0 == 0 && threadIdx.x == 0)      // of how many shares the row is, the next ones holding `share` tiles each
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
         o += f * x[2 + d];
       }
       if (n == tiles) {
-        finish<T, C>(a, b, h * a.group + qt * 16 + r, h, d, o, sum, m);
+        finish<T, C>(a, b, h * a.group + qt * 16 * QT + r, h, d, o, sum, m);
       } else {
         if (d == 0) { parts.ml[(slot + r) * 2] = m; parts.ml[(slot + r) * 2 + 1] = sum; }
         parts.o[(slot + r) * DP + d] = o;
@@ -595,14 +631,14 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
 // Joins the rows that cross a border of shares, one workgroup per row and query.  A long utterance alone leaves a hundred parts
 // of a row, so the maxima are taken by 256 threads at a time and the outputs by as many groups of DP / 4 threads as there are,
 // each with its own parts, in a fixed order.
-template <int T, int C, int DP>
+template <int T, int C, int DP, int QT>
 __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a) {
   constexpr int GROUPS = 256 / (DP / 4);
   __shared__ float red[2][4], weight[256];
   __shared__ taco_f4 outs[GROUPS][DP / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t rows_per = a.n_heads * a.q_tiles;
-  const int held = a.group < 16 ? a.group : 16;
+  const int held = min(a.group, 16 * QT);
   const Partials parts(a, rows_per, held);
   const uint32_t nth = blockIdx.x / held;
   const taco_u2 info = parts.rows[nth];
@@ -610,7 +646,7 @@ __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a)
   if (n == 1) return;
   const uint32_t row = nth % rows_per;
   const int r = blockIdx.x % held, b = nth / rows_per, qt = row % a.q_tiles, h = row / a.q_tiles;
-  if (qt * 16 + r >= a.group) return;
+  if (qt * 16 * QT + r >= a.group) return;
   const auto at = [&](uint32_t k) { return (size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r; };
   float m = NEG_INF;
   for (uint32_t k = tid; k < n; k += 256) m = fmaxf(m, parts.ml[at(k) * 2]);
@@ -645,7 +681,7 @@ __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a)
     float total = 0.0f;
 #pragma unroll
     for (int i = 0; i < GROUPS; ++i) total += outs[i][d / 4][d % 4];
-    finish<T, C>(a, b, h * a.group + qt * 16 + r, h, d, total, sum, m);
+    finish<T, C>(a, b, h * a.group + qt * 16 * QT + r, h, d, total, sum, m);
   }
 }
 
@@ -747,16 +783,18 @@ struct Plan {
   int64_t bytes;
 };
 
-template <int T, int C, int DP>
+template <int T, int C, int DP, int QT>
 int plan_of(Plan& p, int device, int n_cu) {
   // workgroups of this kernel that a CU holds: a grid beyond that would end with a part-filled round
-  static std::atomic<int> known[64][17];
-  p.tt = Attend<T, C, DP>::TT;
+  static std::atomic<int> known[64][16 * QT + 1];
+  p.tt = Attend<T, C, DP, QT>::TT;
   const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
   int per_cu = known[device][p.held].load(std::memory_order_relaxed);
   if (!per_cu) {
-    auto kernel = taco_kv_attend_kernel<T, C, DP>;
-    if (lds > 65536) TACO_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    auto kernel = taco_kv_attend_kernel<T, C, DP, QT>;
+    constexpr int MOST = AT_WAVES * 16 * QT * (DP + 2) * 4;
+    static_assert(MOST <= 160 * 1024, "a CU's LDS");
+    if (MOST > 65536) TACO_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MOST));
     TACO_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, 64 * AT_WAVES, lds));
     if (per_cu < 1) TACO_FAIL(TACO_EINVAL, "taco_kv_attend: the kernel does not fit a CU");
     known[device][p.held].store(per_cu, std::memory_order_relaxed);
@@ -764,21 +802,27 @@ int plan_of(Plan& p, int device, int n_cu) {
   p.workgroups = (uint32_t)(per_cu * n_cu);
   return TACO_OK;
 }
-template <int T, int C, int DP>
+template <int T, int C, int DP, int QT>
 int launch_attend(const AttendParams& a, const Plan& p, hipStream_t s) {
   const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
-  taco_kv_attend_kernel<T, C, DP><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
-  taco_kv_join_kernel<T, C, DP><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a);
+  taco_kv_attend_kernel<T, C, DP, QT><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
+  taco_kv_join_kernel<T, C, DP, QT><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a);
   TACO_HIP(hipGetLastError());
   return TACO_OK;
 }
 
+// The kernel for a call's types, head size and queries per cache head.
 template <typename F>
-int by_types(const taco_kv_cache* c, int dtype, F&& f) {
+int by_types(const taco_kv_cache* c, int dtype, int group, F&& f) {
+  const auto by_group = [&](auto t, auto h, auto d) {
+    if constexpr (h.value != TACO_F32)
+      if (group > 16) return f(t, h, d, std::integral_constant<int, 2>());
+    return f(t, h, d, std::integral_constant<int, 1>());
+  };
   const auto by_dim = [&](auto t, auto h) {
-    if (c->head_dim <= 64) return f(t, h, std::integral_constant<int, 64>());
-    if (c->head_dim <= 128) return f(t, h, std::integral_constant<int, 128>());
-    return f(t, h, std::integral_constant<int, 256>());
+    if (c->head_dim <= 64) return by_group(t, h, std::integral_constant<int, 64>());
+    if (c->head_dim <= 128) return by_group(t, h, std::integral_constant<int, 128>());
+    return by_group(t, h, std::integral_constant<int, 256>());
   };
   using F32 = std::integral_constant<int, TACO_F32>;
   using F16 = std::integral_constant<int, TACO_F16>;
@@ -794,13 +838,14 @@ int by_types(const taco_kv_cache* c, int dtype, F&& f) {
 // Checks the sizes and settles the plan; the device is current.
 int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who, Plan& p) {
   p.group = t->n_q_heads / c->n_heads;
-  p.q_tiles = (p.group + 15) / 16;
-  p.held = p.group < 16 ? p.group : 16;
+  const int at_once = p.group <= 16 || c->dtype == TACO_F32 ? 16 : 32;
+  p.q_tiles = (p.group + at_once - 1) / at_once;
+  p.held = p.group < at_once ? p.group : at_once;
   p.dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   int n_cu;
   int rc = taco_device_check(c->device, &n_cu);
   if (rc != TACO_OK) return rc;
-  rc = by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return plan_of<ty.value, ca.value, dp.value>(p, c->device, n_cu); });
+  rc = by_types(c, t->dtype, p.group, [&](auto ty, auto ca, auto dp, auto qt) { return plan_of<ty.value, ca.value, dp.value, qt.value>(p, c->device, n_cu); });
   if (rc != TACO_OK) return rc;
   const int64_t rows = (int64_t)t->n_seqs * c->n_heads * p.q_tiles;
   const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
@@ -819,7 +864,7 @@ int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const cha
   if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
   if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
   // rows and 16-token tiles are counted in 32 bits
-  if ((int64_t)t->n_seqs * (t->n_q_heads + 16ll * c->n_heads) >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
+  if ((int64_t)t->n_seqs * (t->n_q_heads + 32ll * c->n_heads) >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
     TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads and up to %d pages", who, t->n_seqs, t->n_q_heads, t->table_width);
   return TACO_OK;
 }
@@ -865,7 +910,7 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
   a.n_q_heads = t->n_q_heads; a.head_dim = c->head_dim; a.window = t->window;
   a.group = p.group; a.q_tiles = p.q_tiles; a.workspace = (char*)t->workspace;
   a.workgroups = taco_make_divisor(p.workgroups);
-  return by_types(c, t->dtype, [&](auto ty, auto ca, auto dp) { return launch_attend<ty.value, ca.value, dp.value>(a, p, (hipStream_t)stream); });
+  return by_types(c, t->dtype, p.group, [&](auto ty, auto ca, auto dp, auto qt) { return launch_attend<ty.value, ca.value, dp.value, qt.value>(a, p, (hipStream_t)stream); });
 }
 
 extern "C" int taco_kv_status(const taco_kv_cache* c, void* stream) {
