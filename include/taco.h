@@ -285,7 +285,7 @@ typedef struct taco_kv_append_args {
   const void* k;              /* [n_tokens, n_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
   const void* v;
   const void* q;              /* [n_tokens, n_q_heads, head_dim] or NULL */
-  void* q_out;                /* like q (may be q itself); NULL when q is */
+  void* q_out;                /* like q (may be q itself), its rows apart from each other and from k and v; NULL when q is */
   const int32_t* table;       /* [n_seqs, table_width] */
   const int32_t* past;        /* [n_seqs] tokens of each utterance that the cache holds already */
   const int32_t* offsets;     /* [n_seqs + 1], rising: rows offsets[b] .. offsets[b+1]-1 are utterance b's new tokens;
@@ -309,7 +309,7 @@ int taco_kv_append(const taco_kv_cache* cache, const taco_kv_append_args* args, 
 
 typedef struct taco_kv_attend_args {
   const void* q;              /* [n_seqs, n_q_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
-  void* out;                  /* like q */
+  void* out;                  /* like q (may be q itself), its rows apart from each other */
   float* lse;                 /* [n_seqs, n_q_heads] or NULL */
   const int32_t* table;       /* [n_seqs, table_width] */
   const int32_t* lens;        /* [n_seqs] tokens of each utterance, the new one included */
@@ -366,7 +366,8 @@ int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_s
                        int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
 
 /* y[v] = W x[v] + bias for n_vectors vectors x [n_vectors, x_stride] of type `dtype` (TACO_F32, TACO_F16, TACO_BF16), y
- * [n_vectors, y_stride] of the same type; sums are fp32, rounded once.  W is read once for every 64 vectors. */
+ * [n_vectors, y_stride] of the same type; sums are fp32, rounded once.  y may not overlap x.  W is read again for every 32 vectors (every
+ * 16 of a matrix with few rows). */
 int taco_qmat_multiply(const taco_qmat* m, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t n_vectors,
                        int32_t dtype, void* stream);
 

@@ -64,8 +64,8 @@ class PagedCache:
   ``table[b, t // page_size]``.  ``dtype`` is float32, float16, bfloat16 or float8_e4m3fn; the last holds x / scale with
   one scale per head (``k_scale`` / ``v_scale``, float32 [n_heads], 1 when not given).
 
-  Pages and tables are the caller's to hand out; calls on different streams may overlap as long as they touch different
-  pages."""
+  Pages and tables are the caller's to hand out; calls on different streams may overlap as long as none writes a page that
+  another reads or writes.  Inference only: results carry no gradients."""
 
   def __init__(self, n_pages: int, page_size: int, n_heads: int, head_dim: int, dtype: torch.dtype = torch.float32,
                device: Union[torch.device, str, int] = "cuda", k_scale: Optional[torch.Tensor] = None,
@@ -104,7 +104,7 @@ class PagedCache:
       _check_vector(v_scale, "v_scale", torch.float32, n_heads, self.device)
     elif k_scale is not None or v_scale is not None:
       raise ValueError(f"scales belong to an 8-bit cache, not to {k.dtype}")
-    self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+    self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
     self._flags = torch.zeros(1, dtype=torch.int32, device=self.device)
     p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     self._c = abi.TacoKvCache(
@@ -119,20 +119,36 @@ class PagedCache:
     self._attend_forms: Dict[Tuple, Tuple[bytes, int, torch.Tensor]] = {}
 
   @property
+  def k(self) -> torch.Tensor:
+    return self._k
+
+  @property
+  def v(self) -> torch.Tensor:
+    return self._v
+
+  @property
+  def k_scale(self) -> Optional[torch.Tensor]:
+    return self._k_scale
+
+  @property
+  def v_scale(self) -> Optional[torch.Tensor]:
+    return self._v_scale
+
+  @property
   def n_pages(self) -> int:
-    return self.k.shape[0]
+    return self._k.shape[0]
 
   @property
   def page_size(self) -> int:
-    return self.k.shape[1]
+    return self._k.shape[1]
 
   @property
   def n_heads(self) -> int:
-    return self.k.shape[2]
+    return self._k.shape[2]
 
   @property
   def head_dim(self) -> int:
-    return self.k.shape[3]
+    return self._k.shape[3]
 
   def _rows(self, t: torch.Tensor, name: str, tokens: int, heads: Optional[int]) -> None:
     shape = t.shape
@@ -231,7 +247,7 @@ class PagedCache:
              return_lse: bool = False, out: Optional[torch.Tensor] = None):
     """Attention of one new token per utterance: ``q`` [utterances, query heads, head_dim] over the first ``lens`` (int32
     [utterances]) tokens of each, or the last ``window`` of those; ``scale`` defaults to head_dim ** -0.5.  Query head h
-    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``) and, with
+    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q``) and, with
     ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
     (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
     infinite value that is seen gives NaN."""

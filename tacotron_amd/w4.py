@@ -122,7 +122,8 @@ class W4Matrix:
 
   def matvec(self, x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x W^T + bias for vectors ``x`` [..., in_features] in float32, float16 or bfloat16; the result [..., out_features] has
-    x's type, its sums are fp32 and rounded once.  Meant for a few vectors (the matrix is read once for every 64)."""
+    x's type, its sums are fp32 and rounded once.  ``out`` may not overlap ``x``.  Meant for a few vectors: the matrix is read
+    again for every 32.  Inference only: results carry no gradients."""
     key = (x.shape, x.stride(), x.dtype, x.device) if out is None else \
           (x.shape, x.stride(), x.dtype, x.device, out.shape, out.stride(), out.dtype, out.device)
     form = self._forms.get(key)
@@ -137,8 +138,10 @@ class W4Matrix:
     if out is None:
       out = _lib.new(want)
     if n:
-      rc = self._lib.taco_qmat_multiply(self._ref, x.data_ptr(), x_pitch, out.data_ptr(), y_pitch, n, code,
-                                        _lib.raw_stream(self._c.device))
+      xp, op = x.data_ptr(), out.data_ptr()
+      if xp == op:
+        raise ValueError("out may not be x: every result needs all of its vector")
+      rc = self._lib.taco_qmat_multiply(self._ref, xp, x_pitch, op, y_pitch, n, code, _lib.raw_stream(self._c.device))
       if rc:
         _lib.check(rc)
     return out

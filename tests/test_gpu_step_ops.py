@@ -322,6 +322,7 @@ def test_attend(dtype, held, heads, hq, d, page, lens, window, order):
   into = torch.full((len(lens), hq, d + 16), 7.0, dtype=dtype, device=DEV)
   assert cache.attend(q, table, lens_dev, window=window, out=into[..., :d]) is not None
   assert torch.equal(into[..., :d], got[0]) and bool((into[..., d:] == 7).all())
+  assert cache.attend(q, table, lens_dev, window=window, out=q) is q and torch.equal(q, got[0])      # in place
 
 
 def test_attend_peaked_scores():
@@ -409,6 +410,8 @@ def test_a_cache_beyond_32_bit_offsets():
 def test_refused_tensors():
   from tacotron_amd.paged import PagedCache
   cache = PagedCache(4, 16, 2, 64, dtype=BF16, device=DEV)
+  with pytest.raises(AttributeError):
+    cache.k = cache.v
   assert (cache.n_pages, cache.page_size, cache.n_heads, cache.head_dim) == (4, 16, 2, 64)
   t = lambda *s, dtype=BF16, device=DEV: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
   i = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
@@ -672,7 +675,7 @@ def test_matvec_refusals():
     lambda: W4Matrix.from_codes(packed, scales[:4]), lambda: W4Matrix.from_codes(packed.int(), scales), lambda: W4Matrix.from_codes(packed, scales.double()),
     lambda: W4Matrix.from_codes(packed, scales, zeros=z[:, :1]), lambda: W4Matrix.from_codes(packed, scales, zeros=z.int()),
     lambda: W4Matrix.from_codes(packed, scales, bias=torch.zeros(7, device=DEV)), lambda: W4Matrix.from_codes(packed.cpu(), scales.cpu()),
-    lambda: W.matvec(x[:, :63]), lambda: W.matvec(x.double()), lambda: W.matvec(x.cpu()), lambda: W.matvec(x, out=torch.zeros(2, 9, device=DEV)),
+    lambda: W4Matrix.from_weights(torch.ones(64, 64, device=DEV)).matvec(x, out=x), lambda: W.matvec(x[:, :63]), lambda: W.matvec(x.double()), lambda: W.matvec(x.cpu()), lambda: W.matvec(x, out=torch.zeros(2, 9, device=DEV)),
     lambda: W.matvec(x, out=torch.zeros(8, 2, device=DEV).t()), lambda: W.matvec(x, out=torch.zeros(1, 8, device=DEV).expand(2, 8)),
     lambda: quantize(torch.zeros(3, 0, device=DEV)), lambda: quantize(torch.zeros(3, 8, device=DEV), group=48), lambda: quantize(torch.zeros(3, 8)),
   ):
@@ -728,3 +731,56 @@ def test_layers_of_a_decoder_step(dtype, held):
       x = x.clone()
       x[last] += (y / y.float().abs().mean() * 0.1).to(dtype)
     past = lens
+
+
+def test_matrix_and_step_in_a_graph():
+  """A captured step of one layer (projection, append, attend, projection), replayed with new inputs; every replay equals the
+  eager calls on the same inputs, which run in between."""
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(31)
+  width, hq, hkv, d = 192, 4, 2, 48
+  qkv = hq + 2 * hkv
+  W = [W4Matrix.from_weights(torch.randn(n, k, generator=g, device=DEV).to(BF16), group=64, symmetric=False)
+       for n, k in ((qkv * d, width), (width, hq * d))]
+  caches = [make_cache(12, 32, hkv, d, BF16, gen(8)) for _ in range(2)]
+  table = make_table([4, 4, 3], 12, 4, 5)
+  past = torch.tensor([0, 31, 64], dtype=torch.int32, device=DEV)
+  inv_freq = torch.rand(8, generator=g, device=DEV, dtype=torch.float64)
+  x = torch.zeros(3, width, dtype=BF16, device=DEV)
+
+  def step(cache):
+    h = W[0].matvec(x).view(3, qkv, d)
+    q = cache.append(h[:, hq:hq + hkv], h[:, hq + hkv:], table, past, q=h[:, :hq], inv_freq=inv_freq, interleaved=True)
+    return W[1].matvec(cache.attend(q, table, past + 1).flatten(1))
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    out = step(caches[0])
+  for _ in range(8):
+    x.copy_(torch.randn(3, width, generator=g, device=DEV))
+    graph.replay()
+    want = step(caches[1])
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    past += 1
+  for c in caches:
+    c.check()
+  assert torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)
+
+
+def test_matvec_on_two_streams():
+  """One matrix, two streams at once, each as alone."""
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(33)
+  W = W4Matrix.from_weights(torch.randn(5000, 700, generator=g, device=DEV).to(F16), group=32)
+  xs = [torch.randn(n, 700, generator=g, device=DEV).to(F16) for n in (1, 16)]
+  want = [W.matvec(x) for x in xs]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream(device=DEV) for _ in range(2)]
+  got = []
+  for _ in range(10):
+    for s, x in zip(streams, xs):
+      with torch.cuda.stream(s):
+        got.append(W.matvec(x))
+  torch.cuda.synchronize()
+  for i, y in enumerate(got):
+    assert torch.equal(y, want[i % 2])
