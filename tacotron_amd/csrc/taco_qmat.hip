@@ -39,22 +39,34 @@ struct PackParams {
 };
 
 __global__ __launch_bounds__(256) void taco_qmat_pack_kernel(const PackParams a) {
-  const int64_t words = a.l.row_blocks * a.l.col_blocks * 256, stats = a.l.row_blocks * a.l.groups * 16;
+  // a thread per lane of a block: four words of eight neighbouring columns each, in 16 bytes
+  const int64_t lanes = a.l.row_blocks * a.l.col_blocks * 64, stats = a.l.row_blocks * a.l.groups * 16;
   const int64_t step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += step) {
-    const int64_t block = i / 256, row_block = block / a.l.col_blocks, col_block = block % a.l.col_blocks;
-    const int lane = (int)(i % 256) / 4, j = (int)(i % 4);
-    const int64_t row = row_block * 16 + (lane & 15), col = col_block * 128 + 32 * j + 8 * (lane >> 4);
-    uint32_t w = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < lanes; i += step) {
+    const int64_t block = i / 64, row_block = block / a.l.col_blocks, col_block = block % a.l.col_blocks;
+    const int lane = (int)(i % 64);
+    const int64_t row = row_block * 16 + (lane & 15), col = col_block * 128 + 8 * (lane >> 4);
+    taco_u4 w = {0, 0, 0, 0};
     if (row < a.n_rows) {
       const uint8_t* p = a.codes + row * a.code_stride;
-      for (int e = 0; e < 8; ++e)
-        if (col + e < a.n_cols) {
-          const uint32_t byte = p[(col + e) / 2];
-          w |= (((col + e) & 1) ? byte >> 4 : byte & 15) << (4 * ((e >> 1) + 4 * (e & 1)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t c = col + 32 * j;
+        uint32_t v = 0;       // columns c .. c + 7 in their order
+        if (c + 8 <= a.n_cols) {
+          __builtin_memcpy(&v, p + c / 2, 4);
+        } else {
+          for (int e = 0; e < 8; ++e)
+            if (c + e < a.n_cols) v |= (((e & 1) ? p[(c + e) / 2] >> 4 : p[(c + e) / 2] & 15u) << (4 * e));
         }
+        // even columns to the low half, odd ones to the high half
+        uint32_t even = v & 0x0f0f0f0fu, odd = (v >> 4) & 0x0f0f0f0fu;
+        even = (even | even >> 4) & 0x00ff00ffu;
+        odd = (odd | odd >> 4) & 0x00ff00ffu;
+        w[j] = ((even | even >> 8) & 0xffffu) | (odd | odd >> 8) << 16;
+      }
     }
-    ((uint32_t*)a.packed)[i] = w;
+    ((taco_u4*)a.packed)[i] = w;
   }
   const int64_t given = ((int64_t)a.n_cols + a.group - 1) / a.group;     // groups that the caller's scales have
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < stats; i += step) {
