@@ -25,12 +25,14 @@ def _check(t: torch.Tensor, name: str, shape: Tuple[int, ...], dtypes, device: t
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-  return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+  """``t`` if its rows lie apart and their elements side by side, or a copy (of a matrix with one row for all, say)."""
+  apart = t.shape[0] == 1 or t.stride(0) >= t.shape[1]
+  return t if apart and (t.shape[1] == 1 or t.stride(1) == 1) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _pitch(t: torch.Tensor) -> int:
   """Elements from row to row (a single row may have any stride)."""
-  return max(t.stride(0), t.shape[1])
+  return t.shape[1] if t.shape[0] == 1 else t.stride(0)
 
 
 def quantize(weight: torch.Tensor, group: int = 128, symmetric: bool = True,

@@ -664,6 +664,21 @@ def test_quantize(dtype, scale_dtype, n, k, group, symmetric):
   check_matvec(unpacked.to(DEV), scales, zeros, group, None, x, W.matvec(x))
 
 
+def test_matrices_with_one_row_for_all():
+  """Scales, zero points, codes and weights that are expanded over the rows."""
+  from tacotron_amd.w4 import W4Matrix, quantize
+  codes, packed, scales, z = make_codes(100, 300, 64, F16, True, gen(31))
+  x = torch.randn(3, 300, generator=gen(32), device=DEV).to(F16)
+  make = lambda c, s, zp: W4Matrix.from_codes(c, s, zeros=zp, in_features=300, group=64).matvec(x)  # noqa: E731
+  one = lambda t: t[5:6].expand(t.shape)  # noqa: E731
+  assert torch.equal(make(packed, one(scales), one(z)), make(packed, one(scales).contiguous(), one(z).contiguous()))
+  assert torch.equal(make(one(packed), scales, z), make(one(packed).contiguous(), scales, z))
+  assert torch.equal(make(packed, scales[:, :1].expand(100, 5), z), make(packed, scales[:, :1].repeat(1, 5), z))
+  w = torch.randn(1, 300, generator=gen(33), device=DEV).expand(40, 300)
+  for a, b in zip(quantize(w, 32, False), quantize(w.contiguous(), 32, False)):
+    assert torch.equal(a, b)
+
+
 def test_matvec_refusals():
   from tacotron_amd.w4 import W4Matrix, quantize
   codes, packed, scales, z = make_codes(8, 64, 32, F32, True, gen(1))

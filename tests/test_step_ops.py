@@ -191,3 +191,17 @@ def test_matrices_have_no_cpu_path():
     w4.quantize(torch.zeros(4, 64))
   with pytest.raises(RuntimeError):
     w4.W4Matrix.from_codes(torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2))
+
+
+def test_rows_of_a_matrix():
+  """Rows are read with a stride of a row at least; one row that stands for all is copied."""
+  import torch
+  from tacotron_amd.w4 import _pitch, _rows
+  base = torch.arange(24).view(4, 6)
+  for t in (base, base[:, :5], base[::2], base[:1], base[:, :1], base[:1].expand(4, 6), base[:, :1].expand(4, 6), base.t(), base[:, ::2],
+            base[0, :1].expand(3, 1), base.as_strided((4, 6), (2, 1)), base[:1].expand(1, 6)):
+    rows = _rows(t)
+    assert _pitch(rows) >= rows.shape[1]
+    assert torch.equal(rows.as_strided(rows.shape, (_pitch(rows), 1)), t)
+    assert (rows.shape[0] - 1) * _pitch(rows) + rows.shape[1] <= rows.untyped_storage().nbytes() // 8 - rows.storage_offset()
+  assert _rows(base[:, :5]).data_ptr() == base.data_ptr()
