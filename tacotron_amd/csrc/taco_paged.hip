@@ -160,6 +160,10 @@ constexpr int AT_WAVES = 4;
 constexpr uint32_t LEAST = AT_WAVES;       // tiles of a workgroup at least: one for every wave
 constexpr float NEG_INF = -__builtin_inff();
 
+// The logarithm (base 2) of the weight of a score that equals the maximum.
+template <int T>
+constexpr float weight_shift = T == TACO_F16 ? 15.0f : 0.0f;
+
 // What a wave holds of one (utterance, cache head, up to 16 query heads): the running maximum and sum of the softmax of
 // query column l & 15 (base 2; the sum is this lane's own part of it) and the unnormalised output, transposed:
 // o[blk][e][i] belongs to element blk * 16 * VE + (4 * (l >> 4) + i) * VE + e of that query's head.
@@ -177,7 +181,9 @@ struct State {
 //     loads VE neighbouring elements of each of its own tokens (16 lanes read one row end to end) and element e of all of
 //     them is one operand: for 16-bit types a v_perm per word turns rows into operands.
 // Weights are rounded to the operand type twice, p = hi + lo: one rounding alone would be as large as that of the
-// output itself, and the second product costs nothing while memory is the bound.
+// output itself, and the second product costs nothing while memory is the bound.  For float16 they are relative to the maximum
+// times 2^-15 (the largest weight is 32768, sums and outputs are fp32): float16 ends at 2^-24, and beside a weight of 1 many
+// small ones, which may outweigh it, would be held to 2^-25 only.
 // Measured (both kernels): 64 ragged sequences up to 8191 tokens, 32 query heads over 8 of 128 in bfloat16, 1.24 GB: 224 us = 5.5
 // TB/s; one of 131075 tokens 100 us = 5.4 TB/s; 33 up to 20000 in 8 bits behind a window of 12000, 64 query heads, 0.68 GB: 137 us =
 // 4.9 TB/s.  A large copy reaches 4.7 TB/s on this card.  Sixteen lines up to 3000 frames, 16 heads of 64 in float16, 0.11 GB: 30 us;
@@ -197,6 +203,7 @@ struct Attend {
   static constexpr int VE = C == TACO_F32 ? 4 : C == TACO_E4M3 ? DP / 16 : (DP < 128 ? DP / 16 : 8);   // elements of a load of V
   static constexpr int NB = DP / (16 * VE);
   static constexpr int VW = VE * CB / 4;                       // ... in words
+  static constexpr float SHIFT = weight_shift<T>;
   using St = State<NB, VE>;
 
   // Query operands: for the K operand whose lane holds elements d0 .. of a row, the same elements of query column l & 15.
@@ -345,7 +352,7 @@ struct Attend {
 #pragma unroll
           for (int e = 0; e < VE; ++e) own.o[blk][e] *= f;
       }
-      const float m = own.m == NEG_INF ? 0.0f : own.m;
+      const float m = (own.m == NEG_INF ? 0.0f : own.m) - SHIFT;
 #pragma unroll
       for (int i = 0; i < SUB * 4; ++i) {
         p[t][i] = __builtin_amdgcn_exp2f(p[t][i] - m);
@@ -525,7 +532,7 @@ __device__ __forceinline__ void finish(const AttendParams& a, int b, int head, i
   if (d >= a.head_dim) return;
   o = sum == 0.0f ? 0.0f : o / sum * (C == TACO_E4M3 ? a.v_scale[h] : 1.0f);
   store_out<T>(a.out + (int64_t)b * a.o_st[0] + (int64_t)head * a.o_st[1], d, o);
-  if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
+  if (d == 0 && a.lse) a.lse[(int64_t)b * a.n_q_heads + head] = sum == 0.0f ? NEG_INF : (m - weight_shift<T> + __builtin_amdgcn_logf(sum)) * 0.693147180559945309f;
 }
 // What a part counts for beside the common maximum.
 __device__ __forceinline__ float weight_of(float m_part, float m) { return m_part == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m_part - m); }

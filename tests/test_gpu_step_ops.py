@@ -335,6 +335,29 @@ def test_attend_peaked_scores():
     check_attend(cache, q, table, [500, 33, 1], 0.7, 0, got)
 
 
+@pytest.mark.parametrize("dtype,held", [(F32, F32), (BF16, BF16), (F16, F16), (F16, E4M3)])
+def test_attend_many_small_weights_beside_a_large_one(dtype, held):
+  """One token's score is 15.72 above all others', whose weights are about 2^-22.7 each: what they sum to is seen where the
+  first token's values are zero, and bounded there by its own size."""
+  n, scale = 4000, 1.0
+  cache, q, table, lens = attend_case(dtype, held, 2, 4, 64, 16, [n, 0, 77], 0)
+  k, v = torch.zeros(2, 1, 64, device=DEV), torch.rand(2, 2, 64, generator=gen(5), device=DEV) + 0.5
+  first = v[1].clone()
+  first[:, ::2] = 0
+  pages = table[0, :n // 16].long()
+  cache.k[pages] = k[0].to(held)
+  cache.v[pages] = v[0].to(held)
+  cache.k[table[0, 33].long(), 5] = torch.nn.functional.pad(torch.tensor([7.5], device=DEV), (0, 63)).to(held)       # token 533
+  cache.v[table[0, 33].long(), 5] = first.to(held)
+  k_scale, v_scale = (torch.ones(2, device=DEV) if t is None else t for t in (cache.k_scale, cache.v_scale))
+  q[0] = 0.0
+  q[0, :, 0] = (2.096 / k_scale).repeat_interleave(2).to(dtype)
+  got = cache.attend(q, table, lens, scale=scale, return_lse=True)
+  check_attend(cache, q, table, [n, 0, 77], scale, 0, got)
+  out = got[0][0].float() / v_scale.repeat_interleave(2)[:, None]
+  assert bool((out[:, ::2] > 2.5e-4).all()) and bool((out[:, 1::2] > 0.4).all())
+
+
 def test_attend_bad_entries_and_lengths():
   """A block on a page that is none is not seen; a length beyond the table ends at it, a negative one is 0: all flagged."""
   cache, q, table, lens = attend_case(BF16, BF16, 2, 4, 64, 16, [100, 64, 20], 0)
