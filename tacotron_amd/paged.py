@@ -185,6 +185,7 @@ class PagedCache:
     tokens, rotated likewise: returned, or written to ``out`` (which may be ``q``).  Rows that belong to no utterance are
     left as they were in ``out``.  No two tokens of a call may go to the same place, and ``out`` may overlap no other
     input."""
+    interleaved = bool(interleaved)
     key = (_form(k), _form(v), _form(table), _form(past), None if q is None else _form(q), None if offsets is None else _form(offsets),
            None if inv_freq is None else _form(inv_freq), interleaved, None if out is None else _form(out))
     tail = self._append_forms.get(key)
@@ -225,7 +226,7 @@ class PagedCache:
       self._index(offsets, "offsets", n + 1)
     a = abi.TacoKvAppendArgs(
       k_stride=k.stride()[:2], v_stride=v.stride()[:2], table_stride=table.stride(0), n_tokens=tokens, n_seqs=n,
-      table_width=width, interleaved=bool(interleaved), dtype=abi.DTYPES[k.dtype])
+      table_width=width, interleaved=interleaved, dtype=abi.DTYPES[k.dtype])
     if inv_freq is not None:
       if inv_freq.dim() != 1 or inv_freq.shape[0] % 8 or 2 * inv_freq.shape[0] > self.head_dim:
         raise ValueError(f"inv_freq must have a multiple of 8 frequencies, at most head_dim / 2 = {self.head_dim // 2}, got {tuple(inv_freq.shape)}")
@@ -251,6 +252,7 @@ class PagedCache:
     ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
     (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
     infinite value that is seen gives NaN."""
+    scale, window = None if scale is None else float(scale), int(window)      # numbers: a tensor would stand for itself in the key
     key = (_form(q), _form(table), _form(lens), scale, window, None if out is None else _form(out))
     found = self._attend_forms.get(key)
     qp, op = q.data_ptr(), 0 if out is None else out.data_ptr()
@@ -292,7 +294,8 @@ class PagedCache:
       self._out(out, q)
     a = abi.TacoKvAttendArgs(
       q_stride=q.stride()[:2], out_stride=(heads * self.head_dim, self.head_dim) if out is None else out.stride()[:2],
-      table_stride=table.stride(0), scale=self.head_dim ** -0.5 if scale is None else scale, window=window, n_seqs=n,
+      table_stride=table.stride(0), scale=self.head_dim ** -0.5 if scale is None else scale,
+      window=min(window, 2 ** 31 - 1), n_seqs=n,
       table_width=width, n_q_heads=heads, dtype=abi.DTYPES[q.dtype])
     need = self._lib.taco_kv_attend_workspace(self._ref, C.byref(a))
     if need < 0:

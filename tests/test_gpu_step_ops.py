@@ -358,6 +358,21 @@ def test_attend_many_small_weights_beside_a_large_one(dtype, held):
   assert bool((out[:, ::2] > 2.5e-4).all()) and bool((out[:, 1::2] > 0.4).all())
 
 
+def test_attend_scale_and_window_are_taken_by_value():
+  cache, q, table, lens = attend_case(F32, F32, 2, 4, 64, 16, [50, 20], 0)
+  scale = torch.tensor(0.25)
+  a = cache.attend(q, table, lens, scale=scale)
+  assert torch.equal(a, cache.attend(q, table, lens, scale=0.25))
+  scale.fill_(0.5)
+  b = cache.attend(q, table, lens, scale=scale)
+  assert torch.equal(b, cache.attend(q, table, lens, scale=0.5)) and not torch.equal(a, b)
+  window = torch.tensor(7)
+  c = cache.attend(q, table, lens, window=window)
+  assert torch.equal(c, cache.attend(q, table, lens, window=7))
+  for wide in (50, 2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40 + 3):      # wider than any length
+    assert torch.equal(cache.attend(q, table, lens, window=wide), cache.attend(q, table, lens)), wide
+
+
 def test_attend_bad_entries_and_lengths():
   """A block on a page that is none is not seen; a length beyond the table ends at it, a negative one is 0: all flagged."""
   cache, q, table, lens = attend_case(BF16, BF16, 2, 4, 64, 16, [100, 64, 20], 0)
