@@ -304,7 +304,8 @@ typedef struct taco_kv_append_args {
  * (x c - y s, y c + x s), in fp32, rounded once to the cache's type - for TACO_E4M3 after the division by the head's
  * scale, what is beyond +-448 becoming +-448.  Rows in front of offsets[0] or behind offsets[n_seqs] are left alone in
  * q_out.  A token whose page is not in the table, or whose table entry is no page, is not written and sets a flag.  No two
- * tokens of a call may have the same place (what is stored there is undefined then). */
+ * tokens of a call may have the same place (what is stored there is undefined then), and k, v and q may not lie in the pages
+ * that are written.  At most 2^24 - 1 tokens at once. */
 int taco_kv_append(const taco_kv_cache* cache, const taco_kv_append_args* args, void* stream);
 
 typedef struct taco_kv_attend_args {
@@ -327,7 +328,8 @@ typedef struct taco_kv_attend_args {
  * query head h reads cache head h / (n_q_heads / n_heads).  lse gets the natural logarithm of the softmax's sum.  An
  * utterance without seen tokens (length 0, none left by bad table entries, which set a flag, no score above -inf) gets zeros
  * and -inf.
- * Slots at and behind lens[b] may hold anything.  Statistics and sums are fp32; results do not depend on timing. */
+ * Slots at and behind lens[b] may hold anything.  n_seqs * n_q_heads is at most 2^23 (2^24 - 1 with up to 16 query heads for a
+ * cache head), a table's pages hold fewer than 2^30 tokens.  Statistics and sums are fp32; results do not depend on timing. */
 int taco_kv_attend(const taco_kv_cache* cache, const taco_kv_attend_args* args, void* stream);
 
 /* Bytes of workspace that taco_kv_attend needs for these arguments (its pointers are not looked at), or a negative code.
@@ -340,7 +342,7 @@ int taco_kv_status(const taco_kv_cache* cache, void* stream);
 
 /* A matrix [n_rows, n_cols] of 4-bit codes: W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), zero = 8
  * where there are no zero points.  `packed` holds codes, scales and zero points in the order the kernel reads them, laid out
- * once by taco_qmat_pack. */
+ * once by taco_qmat_pack.  Fewer than 2^26 rows and up to 2^28 columns. */
 typedef struct taco_qmat {
   const void* packed;         /* taco_qmat_bytes() bytes, 16-byte aligned */
   const float* bias;          /* [n_rows] or NULL */
@@ -366,7 +368,7 @@ int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_s
                        int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
 
 /* y[v] = W x[v] + bias for n_vectors vectors x [n_vectors, x_stride] of type `dtype` (TACO_F32, TACO_F16, TACO_BF16), y
- * [n_vectors, y_stride] of the same type; sums are fp32, rounded once.  y may not overlap x.  W is read again for every 32 vectors (every
+ * [n_vectors, y_stride] of the same type; sums are fp32, rounded once (an infinite element gives NaN).  At most 2^20 vectors.  y may not overlap x.  W is read again for every 32 vectors (every
  * 16 of a matrix with few rows). */
 int taco_qmat_multiply(const taco_qmat* m, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t n_vectors,
                        int32_t dtype, void* stream);

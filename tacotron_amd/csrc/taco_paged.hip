@@ -700,6 +700,9 @@ __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a)
 
 // ---- host ----------------------------------------------------------------------------------------------------------
 
+// Workgroups of 256 threads of one launch must be fewer: a grid's threads are counted in 32 bits.
+constexpr int32_t MAX_GRID = 1 << 24;
+
 bool aligned(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // Addresses of rows: base and strides (elements) in multiples of 16 bytes; writes the strides in bytes.
@@ -752,6 +755,7 @@ extern "C" int taco_kv_append(const taco_kv_cache* c, const taco_kv_append_args*
   int rc = check_cache(c, who, t->dtype);
   if (rc != TACO_OK) return rc;
   if (t->n_tokens < 0 || t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d tokens, %d utterances, table width %d", who, t->n_tokens, t->n_seqs, t->table_width);
+  if (t->n_tokens >= MAX_GRID) TACO_FAIL(TACO_EINVAL, "%s: %d tokens at once, at most %d", who, t->n_tokens, MAX_GRID - 1);
   if (!t->offsets && t->n_tokens != t->n_seqs) TACO_FAIL(TACO_EINVAL, "%s: %d tokens for %d utterances without offsets", who, t->n_tokens, t->n_seqs);
   if (t->rot_dim < 0 || t->rot_dim % 16 || t->rot_dim > c->head_dim) TACO_FAIL(TACO_EINVAL, "%s: rot_dim %d is not a multiple of 16 up to head_dim %d", who, t->rot_dim, c->head_dim);
   if (t->rot_dim && !t->inv_freq) TACO_FAIL(TACO_EINVAL, "%s: rot_dim %d without frequencies", who, t->rot_dim);
@@ -848,12 +852,8 @@ int by_types(const taco_kv_cache* c, int dtype, int group, F&& f) {
   return by_dim(BF16(), E4M3());
 }
 
-// Checks the sizes and settles the plan; the device is current.
-int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who, Plan& p) {
-  p.group = t->n_q_heads / c->n_heads;
-  const int at_once = p.group <= 16 || c->dtype == TACO_F32 ? 16 : 32;
-  p.q_tiles = (p.group + at_once - 1) / at_once;
-  p.held = p.group < at_once ? p.group : at_once;
+// The rest of a plan; the device is current.
+int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, Plan& p) {
   p.dp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256;
   int n_cu;
   int rc = taco_device_check(c->device, &n_cu);
@@ -869,15 +869,20 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char
   return TACO_OK;
 }
 
-int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who) {
+// Checks the sizes and settles how the query heads are divided.
+int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const char* who, Plan& p) {
   if (!t) TACO_FAIL(TACO_EINVAL, "%s: NULL argument", who);
   const int rc = check_cache(c, who, t->dtype);
   if (rc != TACO_OK) return rc;
   if (t->n_seqs < 0 || t->table_width < 0) TACO_FAIL(TACO_EINVAL, "%s: %d utterances, table width %d", who, t->n_seqs, t->table_width);
   if (t->n_q_heads < 1 || t->n_q_heads % c->n_heads) TACO_FAIL(TACO_EINVAL, "%s: %d query heads over %d cache heads", who, t->n_q_heads, c->n_heads);
   if ((int64_t)t->table_width * c->page_size >= TACO_KV_MAX_TOKENS) TACO_FAIL(TACO_EINVAL, "%s: %d pages of %d tokens per utterance", who, t->table_width, c->page_size);
-  // rows and 16-token tiles are counted in 32 bits
-  if ((int64_t)t->n_seqs * (t->n_q_heads + 32ll * c->n_heads) >= (1ll << 31) || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
+  p.group = t->n_q_heads / c->n_heads;
+  const int at_once = p.group <= 16 || c->dtype == TACO_F32 ? 16 : 32;
+  p.q_tiles = (p.group + at_once - 1) / at_once;
+  p.held = p.group < at_once ? p.group : at_once;
+  // a workgroup joins each query head (of whole groups of `held`); 16-token tiles are counted in 32 bits
+  if ((int64_t)t->n_seqs * c->n_heads * p.q_tiles * p.held >= MAX_GRID || ((int64_t)t->table_width * c->page_size / 16 + 1) * t->n_seqs >= (1ll << 32))
     TACO_FAIL(TACO_EINVAL, "%s: %d utterances of %d heads and up to %d pages", who, t->n_seqs, t->n_q_heads, t->table_width);
   return TACO_OK;
 }
@@ -886,19 +891,20 @@ int check_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, const cha
 
 extern "C" int64_t taco_kv_attend_workspace(const taco_kv_cache* c, const taco_kv_attend_args* t) {
   const char* who = "taco_kv_attend_workspace";
-  int rc = check_attend(c, t, who);
+  Plan p;
+  int rc = check_attend(c, t, who, p);
   if (rc != TACO_OK) return rc;
   if (t->n_seqs == 0) return 0;
   DeviceScope on_device(c->device);
   TACO_HIP(on_device.status);
-  Plan p;
-  rc = plan_attend(c, t, who, p);
+  rc = plan_attend(c, t, p);
   return rc == TACO_OK ? p.bytes : rc;
 }
 
 extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, void* stream) {
   const char* who = "taco_kv_attend";
-  int rc = check_attend(c, t, who);
+  Plan p;
+  int rc = check_attend(c, t, who, p);
   if (rc != TACO_OK) return rc;
   if (t->window < 0) TACO_FAIL(TACO_EINVAL, "%s: window %d", who, t->window);
   if (!(t->scale - t->scale == 0.0f)) TACO_FAIL(TACO_EINVAL, "%s: scale is not finite", who);
@@ -911,8 +917,7 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
     TACO_FAIL(TACO_EINVAL, "%s: rows must start at multiples of 16 bytes (and not be NULL)", who);
   DeviceScope on_device(c->device);
   TACO_HIP(on_device.status);
-  Plan p;
-  rc = plan_attend(c, t, who, p);
+  rc = plan_attend(c, t, p);
   if (rc != TACO_OK) return rc;
   if ((!t->workspace || !aligned(t->workspace) || t->workspace_bytes < p.bytes)) TACO_FAIL(TACO_EINVAL, "%s: needs a 16-byte aligned workspace of %lld bytes, has %lld", who, (long long)p.bytes, (long long)t->workspace_bytes);
   a.k_pages = (const char*)c->k; a.v_pages = (const char*)c->v; a.k_scale = c->k_scale; a.v_scale = c->v_scale;

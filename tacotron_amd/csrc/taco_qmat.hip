@@ -132,7 +132,8 @@ __global__ __launch_bounds__(64) void taco_qmat_quantize_kernel(const QuantizePa
 
 int check_qmat(const taco_qmat* m, const char* who) {
   if (!m) TACO_FAIL(TACO_EINVAL, "%s: NULL matrix", who);
-  if (m->n_rows < 1 || m->n_cols < 1 || m->n_rows > (1 << 28) || m->n_cols > (1 << 28)) TACO_FAIL(TACO_EINVAL, "%s: %d rows, %d columns", who, m->n_rows, m->n_cols);
+  // (a grid's threads are counted in 32 bits, 64 to a row at most)
+  if (m->n_rows < 1 || m->n_cols < 1 || m->n_rows >= (1 << 26) || m->n_cols > (1 << 28)) TACO_FAIL(TACO_EINVAL, "%s: %d rows, %d columns", who, m->n_rows, m->n_cols);
   if (m->group != 32 && m->group != 64 && m->group != 128) TACO_FAIL(TACO_EINVAL, "%s: group %d is not 32, 64 or 128", who, m->group);
   if (m->scale_dtype != TACO_F32 && m->scale_dtype != TACO_F16 && m->scale_dtype != TACO_BF16) TACO_FAIL(TACO_EINVAL, "%s: scale_dtype %d", who, m->scale_dtype);
   return TACO_OK;

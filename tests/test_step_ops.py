@@ -85,7 +85,7 @@ def test_bad_caches_are_refused(change, word):
 
 
 @pytest.mark.parametrize("change,word", [
-  (dict(n_tokens=-1), "tokens"), (dict(n_seqs=-1), "utterances"), (dict(n_tokens=3), "offsets"), (dict(table_width=-1), "table"),
+  (dict(n_tokens=-1), "tokens"), (dict(n_tokens=1 << 24, offsets=64), "tokens at once"), (dict(n_seqs=-1), "utterances"), (dict(n_tokens=3), "offsets"), (dict(table_width=-1), "table"),
   (dict(rot_dim=8, inv_freq=64), "rot_dim"), (dict(rot_dim=80, inv_freq=64), "rot_dim"), (dict(rot_dim=-16, inv_freq=64), "rot_dim"),
   (dict(rot_dim=32), "frequencies"), (dict(q=4096, n_q_heads=4), "queries"), (dict(q_out=4096, n_q_heads=4), "queries"),
   (dict(q=4096, q_out=4096), "queries"), (dict(table=None), "table"), (dict(past=None), "past"), (dict(k=4098), "16 bytes"),
@@ -103,6 +103,7 @@ def test_bad_appends_are_refused(change, word):
   (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(table_width=1 << 27), "pages"),
   (dict(table=None), "table"), (dict(lens=None), "lens"), (dict(q=4100), "16 bytes"), (dict(out=None), "16 bytes"),
   (dict(out_stride=(512, 63)), "16 bytes"), (dict(n_seqs=1 << 29), "utterances of"),
+  (dict(n_seqs=1 << 21), "utterances of"), (dict(n_seqs=1 << 10, table_width=(1 << 26) - 1), "utterances of"),
 ])
 def test_bad_attends_are_refused(change, word):
   with pytest.raises(_lib.TacoError) as e:
@@ -152,7 +153,7 @@ def test_size_of_a_packed_matrix():
 
 
 @pytest.mark.parametrize("change,word", [
-  (dict(n_rows=0), "rows"), (dict(n_cols=0), "columns"), (dict(n_rows=1 << 29), "rows"), (dict(group=16), "group"), (dict(group=0), "group"),
+  (dict(n_rows=0), "rows"), (dict(n_cols=0), "columns"), (dict(n_rows=1 << 29), "rows"), (dict(n_rows=1 << 26), "rows"), (dict(group=16), "group"), (dict(group=0), "group"),
   (dict(scale_dtype=3), "scale_dtype"), (dict(scale_dtype=-1), "scale_dtype")])
 def test_bad_matrices_are_refused(change, word):
   L, m = _lib.lib(), _qmat(**change)
