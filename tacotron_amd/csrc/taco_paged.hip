@@ -797,6 +797,7 @@ namespace {
 struct Plan {
   int group, q_tiles, held, dp, tt;
   uint32_t workgroups;
+  bool join;
   int64_t bytes;
 };
 
@@ -823,7 +824,7 @@ template <int T, int C, int DP, int QT>
 int launch_attend(const AttendParams& a, const Plan& p, hipStream_t s) {
   const size_t lds = (size_t)AT_WAVES * p.held * (DP + 2) * 4;
   taco_kv_attend_kernel<T, C, DP, QT><<<dim3(p.workgroups), dim3(64 * AT_WAVES), lds, s>>>(a);
-  taco_kv_join_kernel<T, C, DP, QT><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a);
+  if (p.join) taco_kv_join_kernel<T, C, DP, QT><<<dim3((unsigned)(a.n_seqs * a.n_heads * a.q_tiles * p.held)), dim3(256), 0, s>>>(a);
   TACO_HIP(hipGetLastError());
   return TACO_OK;
 }
@@ -862,8 +863,10 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, Plan& p) {
   if (rc != TACO_OK) return rc;
   const int64_t rows = (int64_t)t->n_seqs * c->n_heads * p.q_tiles;
   const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
-  // no more workgroups than there are parts when every row is cut on its own
-  const int64_t most = rows * (((tiles < 1 ? 1 : tiles) + LEAST - 1) / LEAST);
+  // no more workgroups than there are parts when every row is cut on its own; if all of those are there and a table has room for
+  // one part of a row only, every row is finished by its workgroup and the second kernel is left out
+  const int64_t parts = ((tiles < 1 ? 1 : tiles) + LEAST - 1) / LEAST, most = rows * parts;
+  p.join = parts > 1 || most > p.workgroups;
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
   p.bytes = (rows + 1) / 2 * 16 + (int64_t)2 * p.workgroups * p.held * (2 + p.dp) * 4;
   return TACO_OK;

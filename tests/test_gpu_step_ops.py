@@ -307,6 +307,11 @@ ATTENDS = [
   (F16, E4M3, 2, 34, 256, 48, [49, 700], 0, "wide"),
   (BF16, BF16, 8, 32, 128, 64, [20000], 0, "own"),
   (BF16, BF16, 1, 8, 128, 64, [9000, 100, 0, 5000] + [40] * 300, 0, "own"),
+  # tables with room for a part of a row only (128 tokens, 64 in fp32): nothing to join, unless there are more rows than workgroups
+  (BF16, BF16, 4, 8, 64, 16, [112, 1, 0, 97, 64, 33], 0, "own"),
+  (F32, F32, 3, 3, 128, 16, [48, 0, 17, 1], 0, "tokens"),
+  (F16, E4M3, 1, 40, 128, 32, [96, 5], 20, "own"),
+  (BF16, BF16, 8, 16, 128, 64, [64, 3, 50, 0, 33] * 60, 0, "own"),
 ]
 
 
