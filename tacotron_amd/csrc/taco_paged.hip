@@ -157,7 +157,7 @@ struct AttendParams {
 };
 
 constexpr int AT_WAVES = 4;
-constexpr uint32_t LEAST = AT_WAVES;       // tiles of a workgroup at least: one for every wave
+constexpr uint32_t PART = AT_WAVES;        // tiles of a part of a row: one for every wave
 constexpr float NEG_INF = -__builtin_inff();
 
 // The logarithm (base 2) of the weight of a score that equals the maximum.
@@ -417,15 +417,14 @@ struct Attend {
 
 // ---- who does what ----
 // All tiles of a call stand in one line: utterance by utterance, within it row by row (a row: one cache head and up to 16 or
-// 32 of its query heads), within a row from the first seen tile to the last.  The line is cut into equal shares, one per
-// workgroup of a grid that fills the GPU once, whatever the lengths are: a long utterance alone is split over its length,
-// a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is finished
-// by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a second
-// kernel joins in the order of the workgroups.  A workgroup whose share holds the end of one row and the beginning of the next
-// starts twice, 2 to 3 us each.  So where the tiles are so few that every row can be cut into parts of four tiles of its own, one
-// workgroup each, that is done instead (777 tokens of 8 heads of 128: 6 against 10 us).  Joining in the first kernel, by the last
-// workgroup of a row, was slower: what the others wrote has to be stored through to memory and awaited (sixteen lines 35
-// against 31 us, with a fence 211).
+// 32 of its query heads), within a row from the first seen tile to the last, in parts of four tiles, one for each wave.  The line is cut
+// into equal shares of whole parts, one per workgroup of a grid that fills the GPU once, whatever the lengths are: a long utterance alone
+// is split over its length, a batch of short ones is packed, and no workgroup waits for the longest.  A row that lies within one share is
+// finished by its workgroup; of a row that crosses a border every workgroup leaves a partial result (maximum, sum, output), which a
+// second kernel joins in the order of the workgroups.  Shares of any number of tiles were slower where rows are short, because a
+// workgroup's waves wait for each other at a row's end (64 utterances up to 255 tokens, 8 heads of 128: 27.5 us, with whole parts 17.8;
+// up to 1023: 48 and 46.5).  Joining in the first kernel, by the last workgroup of a row, was slower: what the others wrote has to be
+// stored through to memory and awaited (sixteen lines 35 against 31 us, with a fence 211).
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 
 // Inclusive sum over the lanes of a wave (DPP: shifts within rows of 16, then each row's last value to the next one's lanes,
@@ -443,24 +442,20 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
   return add_dpp<0x143, 0xc>(v);   // row_bcast:31
 }
 
-// What a sum over utterances counts, of one row each: tiles, and parts of LEAST tiles.
-struct Count {
-  uint32_t tiles, parts;
-};
-
-// 64 utterances, one per lane: what each sees and how many tiles its rows have.
+// 64 utterances, one per lane: what each sees and of how many parts its rows are.
 template <int TT>
 struct Utterances {
   int base;                  // the first of them
-  Count before;              // of the utterances in front of them
+  uint32_t before;           // parts of a row of each utterance in front of them
   int low, len;              // seen tokens [low, len) of this lane's utterance
-  Count own, scan;           // of its rows (one that sees nothing has a tile, so that somebody writes its zeros); inclusive sum
+  uint32_t tiles;            // of its rows (one that sees nothing has a tile, so that somebody writes its zeros)
+  uint32_t parts, scan;      // of PART tiles each; inclusive sum
 
   __device__ __forceinline__ void load(const AttendParams& a, int first, bool flag) {
     base = first;
     const int b = first + (threadIdx.x & 63);
     len = low = 0;
-    own.tiles = 0;
+    tiles = 0;
     if (b < a.n_seqs) {
       len = a.lens[b];
       const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
@@ -469,45 +464,43 @@ struct Utterances {
         len = len < 0 ? 0 : (int)room;
       }
       low = a.window > 0 ? max(0, len - a.window) : 0;
-      own.tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
+      tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
     }
-    own.parts = (own.tiles + LEAST - 1) / LEAST;
-    scan = {wave_scan(own.tiles), wave_scan(own.parts)};
+    parts = (tiles + PART - 1) / PART;
+    scan = wave_scan(parts);
   }
-  __device__ __forceinline__ Count last() const { return {lane_of(scan.tiles, 63), lane_of(scan.parts, 63)}; }
+  __device__ __forceinline__ uint32_t last() const { return lane_of(scan, 63); }
   // Loads the first 64 and counts all.
-  __device__ __forceinline__ Count load_all(const AttendParams& a, bool flag) {
-    Count sum = {0, 0};
+  __device__ __forceinline__ uint32_t load_all(const AttendParams& a, bool flag) {
+    uint32_t sum = 0;
     for (int i = 64; i < a.n_seqs; i += 64) {
       load(a, i, flag);
-      sum = {sum.tiles + last().tiles, sum.parts + last().parts};
+      sum += last();
     }
     load(a, 0, flag);
-    before = {0, 0};
-    return {sum.tiles + last().tiles, sum.parts + last().parts};
+    before = 0;
+    return sum + last();
   }
   // Moves on to the 64 that utterance `b` is one of.
   __device__ __forceinline__ void move_to(const AttendParams& a, int b) {
     while (b >= base + 64) {
-      before = {before.tiles + last().tiles, before.parts + last().parts};
+      before += last();
       load(a, base + 64, false);
     }
   }
-  // Moves on to the 64 in which unit `at` of all rows lies (N: the unit) and returns its utterance; `at` becomes the unit within it.
-  template <uint32_t Count::*N>
+  // Moves on to the 64 in which part `at` of all rows lies and returns its utterance; `at` becomes the part within it.
   __device__ __forceinline__ int find(const AttendParams& a, uint64_t& at, uint32_t rows_per) {
-    while (at >= (uint64_t)(before.*N + lane_of(scan.*N, 63)) * rows_per) move_to(a, base + 64);
-    const int lane = __popcll(__ballot((uint64_t)(before.*N + scan.*N) * rows_per <= at));      // those that end at or before it
-    at -= (uint64_t)(before.*N + lane_of(scan.*N, lane) - lane_of(own.*N, lane)) * rows_per;
+    while (at >= (uint64_t)(before + last()) * rows_per) move_to(a, base + 64);
+    const int lane = __popcll(__ballot((uint64_t)(before + scan) * rows_per <= at));      // those that end at or before it
+    at -= (uint64_t)(before + lane_of(scan, lane) - lane_of(parts, lane)) * rows_per;
     return base + lane;
   }
 };
 
-// Tiles of a share (the division by the number of workgroups is a multiplication as long as it fits, see taco_divisor).
+// Parts of a share (the division by the number of workgroups is a multiplication as long as it fits, see taco_divisor).
 __device__ __forceinline__ uint64_t share_of(const AttendParams& a, uint64_t all) {
   const uint64_t n = all + a.workgroups.div - 1;
-  const uint64_t share = n < (1u << 30) ? taco_divide((uint32_t)n, a.workgroups) : n / a.workgroups.div;
-  return share < LEAST ? LEAST : share;
+  return n < (1u << 30) ? taco_divide((uint32_t)n, a.workgroups) : n / a.workgroups.div;
 }
 __device__ __forceinline__ uint64_t div64(uint64_t n, uint64_t d) { return (n | d) >> 32 ? n / d : (uint64_t)((uint32_t)n / (uint32_t)d); }
 
@@ -544,39 +537,22 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const uint32_t rows_per = a.n_heads * a.q_tiles;         // rows of an utterance
   Utterances<A::TT> us;
-  const Count count = us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64);
-  uint64_t at, share, left;               // where this workgroup begins, how many tiles it takes
-  uint32_t row, tile0;
-  int b;
-  const uint64_t all_parts = (uint64_t)count.parts * rows_per;
-  const bool apart = all_parts <= gridDim.x;      // every row on its own
-  if (apart) {
-    at = blockIdx.x;
-    if (at >= all_parts) return;
-    b = us.template find<&Count::parts>(a, at, rows_per);
-    const uint32_t parts = lane_of(us.own.parts, b - us.base), tiles = lane_of(us.own.tiles, b - us.base);
-    share = (tiles + parts - 1) / parts;
-    row = (uint32_t)at / parts;
-    tile0 = ((uint32_t)at - row * parts) * (uint32_t)share;
-    if (tile0 >= tiles) return;           // an even cut may need fewer parts
-    left = min((uint32_t)share, tiles - tile0);
-  } else {
-    const uint64_t all = (uint64_t)count.tiles * rows_per;
-    share = share_of(a, all);
-    at = share * blockIdx.x;
-    if (at >= all) return;
-    left = min(share, all - at);
-    b = us.template find<&Count::tiles>(a, at, rows_per);
-    const uint32_t tiles = lane_of(us.own.tiles, b - us.base);
-    row = (uint32_t)div64(at, tiles);
-    tile0 = (uint32_t)(at - (uint64_t)row * tiles);
-  }
+  const uint64_t all = (uint64_t)us.load_all(a, blockIdx.x == 0 && threadIdx.x < 64) * rows_per;
+  const uint64_t share = share_of(a, all);        // parts of a workgroup
+  uint64_t at = share * blockIdx.x;               // where this one begins
+  if (at >= all) return;
+  uint64_t left = min(share, all - at);
+  int b = us.find(a, at, rows_per);
+  const uint32_t first_parts = lane_of(us.parts, b - us.base);
+  uint32_t row = (uint32_t)div64(at, first_parts);
+  uint32_t part0 = (uint32_t)(at - (uint64_t)row * first_parts);
   const int held = min(a.group, 16 * QT);            // queries of a row in LDS and in the partial results
   for (bool first = true; left; first = false) {
     us.move_to(a, b);
     const int low = (int)lane_of(us.low, b - us.base), len = (int)lane_of(us.len, b - us.base);
-    const uint32_t tiles = lane_of(us.own.tiles, b - us.base);
-    const uint32_t n = left < tiles - tile0 ? (uint32_t)left : tiles - tile0;
+    const uint32_t tiles = lane_of(us.tiles, b - us.base), row_parts = lane_of(us.parts, b - us.base);
+    const uint32_t taken = left < row_parts - part0 ? (uint32_t)left : row_parts - part0;
+    const uint32_t tile0 = part0 * PART, n = min(taken * PART, tiles - tile0);
     const int h = a.q_tiles == 1 ? row : row / a.q_tiles, qt = row - h * a.q_tiles;
     typename A::Queries q;
     A::load_q(a, b, h, qt, q);
@@ -612,9 +588,9 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
     const int rows = min(a.group - qt * 16 * QT, 16 * QT);
     // a row that began in an earlier share is this workgroup's first partial result, one that only ends later its second
     const Partials parts(a, rows_per, held);
-    if (tile0 == 0 && threadIdx.x == 0)      // of how many shares the row is, the next ones holding `share` tiles each
-      parts.rows[(size_t)b * rows_per + row] = taco_u2{blockIdx.x, n == tiles ? 1 : 1 + (uint32_t)div64(tiles - n + share - 1, share)};
-    const size_t slot = (size_t)(2 * blockIdx.x + (tile0 ? 0 : 1)) * held;
+    if (part0 == 0 && threadIdx.x == 0)      // of how many shares the row is, the next ones holding `share` parts each
+      parts.rows[(size_t)b * rows_per + row] = taco_u2{blockIdx.x, 1 + (uint32_t)div64(row_parts - taken + share - 1, share)};
+    const size_t slot = (size_t)(2 * blockIdx.x + (part0 ? 0 : 1)) * held;
     for (int i = threadIdx.x; i < rows * DP; i += 64 * AT_WAVES) {
       const int r = i / DP, d = i % DP;
       const float* p = lds + r * (DP + 2);
@@ -628,15 +604,15 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
         sum += f * x[1];
         o += f * x[2 + d];
       }
-      if (n == tiles) {
+      if (taken == row_parts) {
         finish<T, C>(a, b, h * a.group + qt * 16 * QT + r, h, d, o, sum, m);
       } else {
         if (d == 0) { parts.ml[(slot + r) * 2] = m; parts.ml[(slot + r) * 2 + 1] = sum; }
         parts.o[(slot + r) * DP + d] = o;
       }
     }
-    left -= n;
-    tile0 = 0;
+    left -= taken;
+    part0 = 0;
     if (++row == rows_per) { row = 0; ++b; }
   }
 }
@@ -865,7 +841,7 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, Plan& p) {
   const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
   // no more workgroups than there are parts when every row is cut on its own; if all of those are there and a table has room for
   // one part of a row only, every row is finished by its workgroup and the second kernel is left out
-  const int64_t parts = ((tiles < 1 ? 1 : tiles) + LEAST - 1) / LEAST, most = rows * parts;
+  const int64_t parts = ((tiles < 1 ? 1 : tiles) + PART - 1) / PART, most = rows * parts;
   p.join = parts > 1 || most > p.workgroups;
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
   p.bytes = (rows + 1) / 2 * 16 + (int64_t)2 * p.workgroups * p.held * (2 + p.dp) * 4;
