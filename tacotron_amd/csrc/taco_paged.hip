@@ -619,10 +619,10 @@ __global__ __launch_bounds__(64 * AT_WAVES) void taco_kv_attend_kernel(const Att
 
 // Joins the rows that cross a border of shares, one workgroup per row and query.  A long utterance alone leaves a hundred parts
 // of a row, so the maxima are taken by 256 threads at a time and the outputs by as many groups of DP / 4 threads as there are,
-// each with its own parts, in a fixed order.
+// each with its own parts, in a fixed order.  What most rows need, 256 maxima and sums and four parts for each group, is loaded at once.
 template <int T, int C, int DP, int QT>
 __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a) {
-  constexpr int GROUPS = 256 / (DP / 4);
+  constexpr int GROUPS = 256 / (DP / 4), AHEAD = 4;
   __shared__ float red[2][4], weight[256];
   __shared__ taco_f4 outs[GROUPS][DP / 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -637,8 +637,19 @@ __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a)
   const int r = blockIdx.x % held, b = nth / rows_per, qt = row % a.q_tiles, h = row / a.q_tiles;
   if (qt * 16 * QT + r >= a.group) return;
   const auto at = [&](uint32_t k) { return (size_t)(2 * (w0 + k) + (k ? 0 : 1)) * held + r; };
-  float m = NEG_INF;
-  for (uint32_t k = tid; k < n; k += 256) m = fmaxf(m, parts.ml[at(k) * 2]);
+  const int mine = tid / (DP / 4), piece = tid % (DP / 4);
+  const auto ml_of = [&](uint32_t k) { return *(const taco_f2*)(parts.ml + at(k) * 2); };
+  const auto o_of = [&](uint32_t k) { return *(const taco_f4*)(parts.o + at(k) * DP + piece * 4); };
+  taco_f2 own = {NEG_INF, 0.0f};
+  taco_f4 part[AHEAD];
+  const auto load_ahead = [&](uint32_t k0) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) part[i] = o_of(min(k0 + mine + i * GROUPS, n - 1));       // behind the last: it again, without weight
+  };
+  if ((uint32_t)tid < n) own = ml_of(tid);
+  load_ahead(0);
+  float m = own[0];
+  for (uint32_t k = tid + 256; k < n; k += 256) m = fmaxf(m, ml_of(k)[0]);
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
   if (lane == 0) red[0][wave] = m;
@@ -646,19 +657,23 @@ __global__ __launch_bounds__(256) void taco_kv_join_kernel(const AttendParams a)
   m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float sum = 0.0f;
   taco_f4 o = {0, 0, 0, 0};
-  const int mine = tid / (DP / 4), piece = tid % (DP / 4);
   for (uint32_t k0 = 0; k0 < n; k0 += 256) {
-    if (k0) __syncthreads();
-    const uint32_t k = k0 + tid;
-    if (k < n) {
-      const float f = weight_of(parts.ml[at(k) * 2], m);
-      weight[tid] = f;
-      sum += f * parts.ml[at(k) * 2 + 1];
+    if (k0) {
+      __syncthreads();
+      if (k0 + tid < n) own = ml_of(k0 + tid);
+      load_ahead(k0);
+    }
+    if (k0 + tid < n) {
+      weight[tid] = weight_of(own[0], m);
+      sum += weight[tid] * own[1];
     }
     __syncthreads();
     const uint32_t here = n - k0 < 256 ? n - k0 : 256;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if ((uint32_t)(mine + i * GROUPS) < here) o += weight[mine + i * GROUPS] * part[i];
 #pragma unroll 4
-    for (uint32_t j = mine; j < here; j += GROUPS) o += weight[j] * *(const taco_f4*)(parts.o + at(k0 + j) * DP + piece * 4);
+    for (uint32_t j = mine + AHEAD * GROUPS; j < here; j += GROUPS) o += weight[j] * o_of(k0 + j);
   }
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, 64);

@@ -7,6 +7,7 @@
 
 #include "taco_internal.h"
 
+typedef float taco_f2 __attribute__((ext_vector_type(2)));
 typedef float taco_f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 taco_bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 taco_bf2 __attribute__((ext_vector_type(2)));
