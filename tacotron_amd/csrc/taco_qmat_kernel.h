@@ -59,11 +59,13 @@ struct Operand<TACO_F32, ODD> {
     for (int n = 0; n < 3; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        // the upper halves of two floats side by side: two bfloat16, cut off
-        v[n][i] = __builtin_amdgcn_perm(__float_as_uint(f[2 * i + 1]), __float_as_uint(f[2 * i]), 0x07060302u);
+        // the upper halves of two floats side by side: two bfloat16, cut off (in the order in which the codes come, see widen)
+        constexpr int FIRST[4] = {0, 2, 1, 3};
+        float &a = f[FIRST[i]], &b = f[FIRST[i] + 4];
+        v[n][i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
         if (n < 2) {
-          f[2 * i] -= __uint_as_float(__float_as_uint(f[2 * i]) & 0xffff0000u);
-          f[2 * i + 1] -= __uint_as_float(__float_as_uint(f[2 * i + 1]) & 0xffff0000u);
+          a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+          b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
         }
       }
   }
@@ -78,9 +80,9 @@ struct Operand<TACO_F32, ODD> {
 // float16's lowest bits, the subnormal c * 2^-24, would need nothing taken off, but the matrix cores lose bits of sums of
 // such products: 2^-15 of the result measured.)
 // Bound by reading the codes: 28672 x 8192 for one bfloat16 vector, 122 MB, takes 26.4 us = 4.6 TB/s (a large copy reaches 4.7; the
-// same loads without any product 23.7 us); groups of 32 columns 35 us, where scaling the sums binds; fp32 vectors 52 us, where
-// splitting them and converting the codes does.  4096 x 4096 4.4 us, 4096 x 1558 for sixteen fp32 vectors 6.4 us, 80 x 1558 for one
-// 5.0 us: the launch, one round trip to memory and, for the last two, a block's chain of products.
+// same loads without any product 23.7 us); groups of 32 columns 35 us, where scaling the sums binds; an fp32 vector 45 us
+// (groups of 64), where splitting it and converting the codes does (a byte at a time 54).  4096 x 4096 4.4 us, 4096 x 1558 for sixteen fp32 vectors 6.1 us, 80 x 1558 for one
+// 5.1 us: the launch, one round trip to memory and, for the last two, a block's chain of products.
 template <int T, int MT, int RT, int GPB, int S, bool ZEROS, bool ODD>
 struct Multiply {
   static constexpr int SB = taco_size_of<S>;
@@ -142,16 +144,18 @@ struct Multiply {
 #pragma unroll
       for (int m = 0; m < MT; ++m) x[j][m].load_end(xr[m], kb * 128 + 32 * j + 8 * g, n_cols);
   }
-  // A word's codes as four words of operands: columns 0, 1, then 2, 3, ..  For fp32 vectors they are converted, a byte at a time
-  // (a small whole number's upper half is its bfloat16): the 16 would triple the rounding errors of the sums, which nothing
-  // hides there (8249 x 9077: 1.1e-6 of the result with it).
+  // A word's codes as four words of operands: columns 0, 1, then 2, 3, ..  For fp32 vectors two at a time are converted from 8-bit
+  // floats of 3 mantissa bits, whose smallest values, the bytes 0 .. 15, are that many times 2^-9: the 16 would triple the rounding
+  // errors of the sums, which nothing hides there (8249 x 9077: 1.1e-6 of the result with it).  Those pairs are columns 0, 4, then 2, 6,
+  // 1, 5 and 3, 7, and the vectors are taken in that order.
+  template <int HALF>
+  static __device__ __forceinline__ uint32_t bytes(uint32_t w) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 512.0f, HALF));
+  }
   static __device__ __forceinline__ taco_u4 widen(uint32_t w, uint32_t mask, uint32_t sixteen) {
     if constexpr (T == TACO_F32) {
       const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;     // columns 0, 4, 1, 5 and 2, 6, 3, 7
-      const auto pair = [](uint32_t bytes, int first, int second) {
-        return __builtin_amdgcn_perm(__float_as_uint((float)((bytes >> (8 * second)) & 255u)), __float_as_uint((float)((bytes >> (8 * first)) & 255u)), 0x07060302u);
-      };
-      return taco_u4{pair(lo, 0, 2), pair(hi, 0, 2), pair(lo, 1, 3), pair(hi, 1, 3)};
+      return taco_u4{bytes<0>(lo), bytes<0>(hi), bytes<1>(lo), bytes<1>(hi)};
     } else if constexpr (T == TACO_BF16) {
       return taco_u4{((w << 3) & mask) | sixteen, ((w >> 1) & mask) | sixteen, ((w >> 5) & mask) | sixteen, ((w >> 9) & mask) | sixteen};
     } else {
