@@ -368,8 +368,8 @@ int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_s
                        int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
 
 /* y[v] = W x[v] + bias for n_vectors vectors x [n_vectors, x_stride] of type `dtype` (TACO_F32, TACO_F16, TACO_BF16), y
- * [n_vectors, y_stride] of the same type; sums are fp32, rounded once (an infinite element gives NaN).  At most 2^20 vectors.  y may not overlap x.  W is read again for every 32 vectors (every
- * 16 of a matrix with few rows). */
+ * [n_vectors, y_stride] of the same type; sums are fp32, rounded once (an infinite element gives NaN).  At most 2^20 vectors.  y may not overlap x.  W is read again
+ * for every 32 vectors (for every 16 of a matrix with few rows or of fp32 vectors). */
 int taco_qmat_multiply(const taco_qmat* m, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t n_vectors,
                        int32_t dtype, void* stream);
 

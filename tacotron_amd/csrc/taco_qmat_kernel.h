@@ -329,22 +329,36 @@ int launch(const taco_qmat_multiply_params& a, hipStream_t s) {
   return TACO_OK;
 }
 
-// How many row blocks a workgroup takes.  Few rows: one workgroup of 16 waves per CU, so that a row block's columns are read by as
-// many waves as possible (bfloat16, one vector, us with 1 x 16 / 2 x 16 / 4 x 8 row blocks x waves: 4096 x 4096 4.6 / 6.6 / 7.1, 8192 x
-// 8192 11.6 / 9.6 / 12.4).  Many rows: each piece of the vectors that is read serves four row blocks (14336 x 4096 with sixteen
-// vectors 22 / 14 / 9.7, 28672 x 8192 with one 40 / 35 / 29).  Groups of 32 columns leave too few registers for four row blocks
-// with fp32 scales, and for 16 waves with two.  More than 16 vectors take two tiles of 16 at a time (28672 x 8192
-// with 32: 73 us with two row blocks, 110 with one) unless the row blocks of all tiles have a CU each (20 x 12559 with 34: 69 us as
-// two tiles, 24 as one each).
+// How many row blocks a workgroup takes, and whether one or two tiles of 16 vectors.  Blocks of rows times tiles that have a CU each:
+// one workgroup of 16 waves per CU, so that a row block's columns are read by as many waves as possible (bfloat16, one vector, us with
+// 1 x 16 / 2 x 16 / 4 x 8 row blocks x waves: 4096 x 4096 4.6 / 6.6 / 7.1, 8192 x 8192 11.6 / 9.6 / 12.4).  More than two to a CU: each
+// piece of the vectors that is read serves four row blocks (14336 x 4096 with sixteen vectors 22 / 14 / 9.7, 28672 x 8192 with one 40 /
+// 35 / 29).  Groups of 32 columns leave too few registers for four row blocks with fp32 scales, and for 16 waves with two.
+// More than 16 vectors of a 16-bit type take two tiles at a time: with two row blocks reading the vectors would bind (28672 x 4096 with
+// 32: 43 us, with four 26; 9000 x 4096 21.7 and 13.5), with one every CU is busy sooner (4096 x 4096 with 32: 11.6 with two, 10.2 with
+// one; not in groups of 32, 4096 x 4097 19.5 and 22.1).  fp32 vectors need three times the registers and take a tile at a time (28672 x
+// 4096 with 32: 50 us, two tiles and two row blocks 80), two only where four row blocks have no room (groups of 32, 28672 x 4096
+// with 17: 73 and 81).
 template <int T, int GPB, int S>
 int launch(const taco_qmat_multiply_params& a, int n_cu, hipStream_t s) {
   constexpr bool FOUR = !(GPB == 4 && S == TACO_F32);
   constexpr int WAVES = GPB == 4 ? 8 : 16;
-  const int row_blocks = (a.n_rows + 15) / 16;
-  if ((int64_t)row_blocks * ((a.n_vectors + 15) / 16) <= n_cu) return launch<T, 1, 1, 16, GPB, S>(a, s);
-  if (a.n_vectors > 16) return launch<T, 2, 2, 8, GPB, S>(a, s);
-  if constexpr (FOUR)
-    if (row_blocks > 2 * n_cu) return launch<T, 1, 4, 8, GPB, S>(a, s);
+  const int64_t row_blocks = (a.n_rows + 15) / 16;
+  int64_t blocks = row_blocks * ((a.n_vectors + 15) / 16);
+  if (blocks <= n_cu) return launch<T, 1, 1, 16, GPB, S>(a, s);
+  if constexpr (T != TACO_F32)
+    if (a.n_vectors > 16) {
+      blocks = row_blocks * ((a.n_vectors + 31) / 32);
+      if constexpr (GPB < 4)
+        if (blocks <= n_cu) return launch<T, 2, 1, 8, GPB, S>(a, s);
+      if constexpr (FOUR)
+        if (blocks > 2 * n_cu) return launch<T, 2, 4, 8, GPB, S>(a, s);
+      return launch<T, 2, 2, 8, GPB, S>(a, s);
+    }
+  if (blocks > 2 * n_cu) {
+    if constexpr (FOUR) return launch<T, 1, 4, 8, GPB, S>(a, s);
+    else if (T == TACO_F32 && a.n_vectors > 16) return launch<T, 2, 2, 8, GPB, S>(a, s);
+  }
   return launch<T, 1, 2, WAVES, GPB, S>(a, s);
 }
 template <int T, int GPB>

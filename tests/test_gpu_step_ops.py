@@ -636,6 +636,14 @@ MATVECS = [
   (BF16, BF16, 7, 8200, 2500, 128, True, True),
   (F32, F32, 16, 8209, 160, 64, False, True),
   (F16, F16, 20, 9001, 130, 32, False, False),
+  # more than a tile of vectors, in each of them
+  (F16, F16, 33, 2000, 129, 128, True, False),
+  (BF16, F32, 30, 4000, 511, 32, True, True),
+  (F16, F32, 64, 4100, 640, 64, False, True),
+  (BF16, BF16, 45, 8200, 301, 64, True, False),
+  (F16, F32, 17, 9001, 200, 32, True, False),
+  (F32, F32, 33, 3000, 300, 64, True, True),
+  (F32, F16, 40, 4100, 257, 128, False, False),
 ]
 
 
