@@ -24,7 +24,7 @@ _MOST_FORMS = 256
 
 
 def _form(t: torch.Tensor) -> Tuple:
-  return t.shape, t.stride(), t.dtype, t.device
+  return t.shape, t.stride(), t.dtype, t.get_device()
 
 
 def _device(device: Union[torch.device, str, int]) -> torch.device:

@@ -126,8 +126,8 @@ class W4Matrix:
     """x W^T + bias for vectors ``x`` [..., in_features] in float32, float16 or bfloat16; the result [..., out_features] has
     x's type, its sums are fp32 and rounded once (an infinite element gives NaN).  ``out`` may not overlap ``x``.  Meant for a few vectors: the matrix is read
     again for every 32 (every 16 in float32).  Inference only: results carry no gradients."""
-    key = (x.shape, x.stride(), x.dtype, x.device) if out is None else \
-          (x.shape, x.stride(), x.dtype, x.device, out.shape, out.stride(), out.dtype, out.device)
+    key = (x.shape, x.stride(), x.dtype, x.get_device()) if out is None else \
+          (x.shape, x.stride(), x.dtype, x.get_device(), out.shape, out.stride(), out.dtype, out.get_device())
     form = self._forms.get(key)
     if form is None:
       form = self._form(x, out)
