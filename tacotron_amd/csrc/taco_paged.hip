@@ -187,7 +187,7 @@ struct State {
 // Measured (both kernels): 64 ragged sequences up to 8191 tokens, 32 query heads over 8 of 128 in bfloat16, 1.24 GB: 224 us = 5.5
 // TB/s; one of 131075 tokens 100 us = 5.4 TB/s; 33 up to 20000 in 8 bits behind a window of 12000, 64 query heads, 0.68 GB: 137 us =
 // 4.9 TB/s.  A large copy reaches 4.7 TB/s on this card.  Sixteen lines up to 3000 frames, 16 heads of 64 in float16, 0.11 GB: 30 us;
-// a lone line of 777 frames in fp32 9.2 us, mostly two launches and four dependent round trips to memory.
+// a lone line of 777 frames in fp32 9.2 us, mostly two launches and five dependent round trips to memory.
 // K and V serve 16 * QT query heads of a cache head; further ones read them again.  With more than 16, QT = 2 pays where reading
 // is the bound (16 x 16384 tokens, 2 heads of 128 in bfloat16, 64 query heads: 82 us with QT = 1, 71 with 2; 16 x 60000 tokens
 // of 64 elements, 64 query heads over one: 144 and 90), not for fp32, whose products are slower than its reading (48 query
