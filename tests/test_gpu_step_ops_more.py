@@ -1,0 +1,74 @@
+"""The self-attention step's operators on the GPU, continued: every form of the kernels, the ends of the range of numbers, calls
+that meet each other.  Tolerances as in test_gpu_step_ops.py."""
+
+import pytest
+import torch
+
+from matvec_bounds import fp32_rms_bound, rms_error
+from test_gpu_step_ops import BF16, DEV, F16, F32, check_matvec, gen, make_codes
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- products -----------------------------------------------------------------------------------------------------------
+
+
+def product_64(codes, scales, zeros, group, x):
+  k = codes.shape[1]
+  spread = lambda t: t.double().repeat_interleave(group, 1)[:, :k]  # noqa: E731
+  return x.double() @ ((codes.double() - (8.0 if zeros is None else spread(zeros))) * spread(scales)).t()
+
+
+# vectors, rows: up to a row block per CU, up to two, more; the same with more than a tile of vectors (256 CUs)
+FORMS = [(1, 40), (3, 4200), (2, 8300), (20, 2100), (20, 4200), (33, 8300)]
+
+
+@pytest.mark.parametrize("scale_dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_every_form_of_the_product(dtype, group, scale_dtype):
+  """Each way of dividing rows and vectors, with and without zero points, vectors at even and at odd addresses."""
+  from tacotron_amd.w4 import W4Matrix
+  k = 300
+  for vectors, n in FORMS:
+    for zeros in (False, True):
+      g = gen(n + group)
+      codes, packed, scales, z = make_codes(n, k, group, scale_dtype, zeros, g)
+      W = W4Matrix.from_codes(packed, scales, zeros=z, in_features=k, group=group)
+      x = torch.randn(vectors, k, generator=g, device=DEV).to(dtype)
+      got = W.matvec(x)
+      check_matvec(codes, scales, z, group, None, x, got)
+      if dtype == F32:
+        assert rms_error(got, product_64(codes, scales, z, group, x)) <= fp32_rms_bound(group, scales.shape[1], zeros), (vectors, n, zeros)
+      wide = torch.full((vectors, k + 3), float("nan"), dtype=dtype, device=DEV)
+      wide[:, 1:k + 1] = x
+      assert torch.equal(W.matvec(wide[:, 1:k + 1]), got), (vectors, n, zeros)
+
+
+@pytest.mark.parametrize("n,k,vectors,group,zeros", [
+  (80, 1558, 1, 32, False), (4096, 1558, 16, 64, False), (8249, 9077, 1, 128, False), (33, 127, 65, 32, True), (4100, 257, 40, 128, True),
+  (100, 20000, 3, 64, True)])
+def test_fp32_products_keep_their_bits(n, k, vectors, group, zeros):
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(n + k)
+  codes, packed, scales, z = make_codes(n, k, group, F32, zeros, g)
+  x = torch.randn(vectors, k, generator=g, device=DEV)
+  got = W4Matrix.from_codes(packed, scales, zeros=z, in_features=k, group=group).matvec(x)
+  assert rms_error(got, product_64(codes, scales, z, group, x)) <= fp32_rms_bound(group, scales.shape[1], zeros)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_as_many_vectors_as_there_may_be(dtype):
+  """2^20 vectors of a small matrix: a launch's second dimension at its largest."""
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(3)
+  codes, packed, scales, z = make_codes(16, 32, 32, F32, True, g)
+  W = W4Matrix.from_codes(packed, scales, zeros=z, group=32)
+  x = torch.randn(1 << 20, 32, generator=g, device=DEV).to(dtype)
+  got = W.matvec(x)
+  for rows in (slice(0, 1 << 12), slice((1 << 19) - 100, (1 << 19) + 100), slice((1 << 20) - (1 << 12), 1 << 20)):
+    check_matvec(codes, scales, z, 32, None, x[rows], got[rows])
+  assert bool(torch.isfinite(got).all())
+
+
+# ---- attend -------------------------------------------------------------------------------------------------------------

@@ -1,0 +1,39 @@
+"""The self-attention step's operators without a GPU, continued: what a build depends on, and the bounds that the GPU tests use."""
+import pytest
+import torch
+
+from matvec_bounds import fp32_rms_bound, rms_error
+
+
+def cut(x, parts):
+  """What `parts` bfloat16, each the leading 8 bits of what the ones before left, hold of fp32 numbers."""
+  held, rest = torch.zeros_like(x), x.clone()
+  for _ in range(parts):
+    part = (rest.view(torch.int32) & -65536).view(torch.float32)
+    held, rest = held + part, rest - part
+  return held
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("n,k,vectors", [(80, 1558, 1), (300, 512, 16), (33, 127, 65)])
+def test_the_bound_of_fp32_products_tells_lost_bits(group, zeros, n, k, vectors):
+  """Products with plain fp32 sums keep the bound; vectors of two parts instead of three, of float16, and results of float16 do not."""
+  g = torch.Generator().manual_seed(n + group)
+  groups = -(-k // group)
+  spread = lambda t: t.repeat_interleave(group, 1)[:, :k]  # noqa: E731
+  c = torch.randint(0, 16, (n, k), generator=g).double()
+  z = torch.randint(0, 16, (n, groups), generator=g).double() if zeros else torch.full((n, groups), 8.0).double()
+  s = torch.rand(n, groups, generator=g) * 0.1 + 0.01
+  w = (c - spread(z)) * spread(s.double())
+  x = torch.randn(vectors, k, generator=g)
+  want = x.double() @ w.t()
+  bound = fp32_rms_bound(group, groups, zeros)
+  sums = torch.zeros(vectors, n)
+  for i in range(groups):
+    at = slice(i * group, min(k, (i + 1) * group))
+    sums += s[:, i] * (x[:, at] @ c[:, at].float().t() - z[:, i].float() * x[:, at].sum(1, keepdim=True))
+  assert rms_error(sums, want) <= bound
+  assert torch.equal(cut(x, 3), x)
+  for wrong in (cut(x, 2).double() @ w.t(), x.half().double() @ w.t(), want.half()):
+    assert rms_error(wrong, want) > 2 * bound
