@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from matvec_bounds import fp32_rms_bound, rms_error
-from test_gpu_step_ops import BF16, DEV, F16, F32, check_matvec, gen, make_codes
+from test_gpu_step_ops import BF16, DEV, E4M3, F16, F32, attend_case, check_attend, check_matvec, gen, make_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,37 @@ def test_as_many_vectors_as_there_may_be(dtype):
 
 
 # ---- attend -------------------------------------------------------------------------------------------------------------
+
+EDGES = [0, 1, 15, 16, 17, 33, 64, 65, 128, 129, 300]
+INSTANCES = [
+  # dtype, cache, heads, query heads, d, page, lens, window, order: types and head sizes with more than 16 query heads a cache head, and without
+  (F16, F16, 2, 40, 64, 16, EDGES, 0, "own"),
+  (F16, F16, 1, 5, 256, 32, EDGES, 40, "tokens"),
+  (F16, F16, 2, 50, 256, 16, EDGES, 0, "heads"),
+  (F16, F16, 1, 17, 144, 48, [700, 5], 0, "own"),
+  (F16, F16, 2, 34, 128, 16, EDGES, 0, "wide"),
+  (BF16, BF16, 2, 64, 128, 64, EDGES, 0, "own"),
+  (BF16, BF16, 2, 48, 256, 16, EDGES, 0, "own"),
+  (BF16, BF16, 1, 33, 208, 32, [1000, 0, 31], 130, "wide"),
+  (BF16, BF16, 1, 71, 128, 16, [2000, 3], 0, "tokens"),
+  (BF16, BF16, 3, 9, 64, 16, EDGES, 0, "own"),
+  (F16, E4M3, 2, 66, 64, 32, EDGES, 0, "own"),
+  (F16, E4M3, 3, 6, 128, 16, EDGES, 20, "tokens"),
+  (F16, E4M3, 1, 4, 256, 16, EDGES, 0, "own"),
+  (F16, E4M3, 1, 20, 112, 16, EDGES, 0, "own"),
+  (BF16, E4M3, 4, 8, 64, 16, EDGES, 0, "heads"),
+  (BF16, E4M3, 1, 24, 48, 16, EDGES, 0, "own"),
+  (BF16, E4M3, 2, 40, 128, 32, EDGES, 65, "own"),
+  (BF16, E4M3, 2, 36, 256, 48, EDGES, 0, "wide"),
+  (F32, F32, 2, 34, 64, 16, EDGES, 0, "own"),
+  (F32, F32, 1, 3, 160, 16, EDGES, 0, "tokens"),
+]
+
+
+@pytest.mark.parametrize("dtype,held,heads,hq,d,page,lens,window,order", INSTANCES)
+def test_every_form_of_the_attention(dtype, held, heads, hq, d, page, lens, window, order):
+  cache, q, table, lens_dev = attend_case(dtype, held, heads, hq, d, page, lens, window, order)
+  got = cache.attend(q, table, lens_dev, window=window, return_lse=True)
+  cache.check()
+  check_attend(cache, q, table, lens, d ** -0.5, window, got)
+  assert cache.attend(q, table, lens_dev, window=window, out=q) is q and torch.equal(q, got[0])
