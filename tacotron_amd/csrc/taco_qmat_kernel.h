@@ -79,6 +79,9 @@ struct Operand<TACO_F32, ODD> {
 // zero points all of it is one such product, of -24.  (A code in a
 // float16's lowest bits, the subnormal c * 2^-24, would need nothing taken off, but the matrix cores lose bits of sums of
 // such products: 2^-15 of the result measured.)
+// A group's sums are formed before its scale makes them small: up to 31 * 128 times the largest element for bfloat16, 15 * 128 for
+// fp32.  So that they stay below the largest fp32 number whatever the vectors, bfloat16 and fp32 codes are held 2^-12 times as large and
+// the finished sum is multiplied by 2^12 (float16 vectors end at 65504).  Both are exact, down to products of 2^-149.
 // Bound by reading the codes: 28672 x 8192 for one bfloat16 vector, 122 MB, takes 26.4 us = 4.6 TB/s (a large copy reaches 4.7; the
 // same loads without any product 23.7 us); groups of 32 columns 35 us, where scaling the sums binds; an fp32 vector 45 us
 // (groups of 64), where splitting it and converting the codes does (a byte at a time 54).  4096 x 4096 4.4 us, 4096 x 1558 for sixteen fp32 vectors 6.1 us, 80 x 1558 for one
@@ -87,6 +90,7 @@ template <int T, int MT, int RT, int GPB, int S, bool ZEROS, bool ODD>
 struct Multiply {
   static constexpr int SB = taco_size_of<S>;
   static constexpr int KIND = T == TACO_F16 ? TACO_F16 : TACO_BF16;       // of the products
+  static constexpr float UNIT = T == TACO_F16 ? 1.0f : 0x1p-12f;          // what a code of 1 is held as
   struct Constants {
     uint32_t mask, sixteen, offset;
   };
@@ -150,7 +154,7 @@ struct Multiply {
   // 1, 5 and 3, 7, and the vectors are taken in that order.
   template <int HALF>
   static __device__ __forceinline__ uint32_t bytes(uint32_t w) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 512.0f, HALF));
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 512.0f * UNIT, HALF));
   }
   static __device__ __forceinline__ taco_u4 widen(uint32_t w, uint32_t mask, uint32_t sixteen) {
     if constexpr (T == TACO_F32) {
@@ -253,10 +257,10 @@ __global__ __launch_bounds__(64 * NW) void taco_qmat_multiply_kernel(const taco_
     for (int m = 0; m < MT; ++m) y[t][m] = taco_f4{0, 0, 0, 0};
   // constants the compiler does not know, so that it keeps them in registers: shift, v_and_or_b32 with both
   typename K::Constants k;
-  if constexpr (K::KIND == TACO_BF16) asm("v_mov_b32 %0, 0x780078\n\tv_mov_b32 %1, 0x41804180" : "=&v"(k.mask), "=v"(k.sixteen));
+  if constexpr (K::KIND == TACO_BF16) asm("v_mov_b32 %0, 0x780078\n\tv_mov_b32 %1, 0x3b803b80" : "=&v"(k.mask), "=v"(k.sixteen));
   else asm("v_mov_b32 %0, 0x3c003c0\n\tv_mov_b32 %1, 0x4c004c00" : "=&v"(k.mask), "=v"(k.sixteen));
-  if constexpr (T == TACO_F32) k.offset = ZEROS ? 0xbf80bf80u : 0xc100c100u;               // -1, -8
-  else if constexpr (T == TACO_BF16) k.offset = ZEROS ? 0xc180c180u : 0xc1c0c1c0u;         // -16, -24
+  if constexpr (T == TACO_F32) k.offset = ZEROS ? 0xb980b980u : 0xbb00bb00u;               // -1, -8 (times UNIT)
+  else if constexpr (T == TACO_BF16) k.offset = ZEROS ? 0xbb80bb80u : 0xbbc0bbc0u;         // -16, -24
   else k.offset = ZEROS ? 0xcc00cc00u : 0xce00ce00u;
   if (wave < whole) {
     // The next block and its piece of the vectors come while this one is multiplied.  Every turn makes the same loads (the last
@@ -302,6 +306,7 @@ __global__ __launch_bounds__(64 * NW) void taco_qmat_multiply_kernel(const taco_
 #pragma unroll
     for (int n = 0; n < NW; ++n) total += part[n][v][row];
     const int64_t n = row_block * 16 + row;
+    total *= 1.0f / K::UNIT;
     if (n < a.n_rows && v0 + v < a.n_vectors) {
       if (a.bias) total += a.bias[n];
       char* out = a.y + (int64_t)(v0 + v) * a.y_stride;

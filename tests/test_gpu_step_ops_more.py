@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from matvec_bounds import fp32_rms_bound, rms_error
-from test_gpu_step_ops import BF16, DEV, E4M3, F16, F32, attend_case, check_attend, check_matvec, gen, make_codes
+from test_gpu_step_ops import BF16, DEV, E4M3, F16, F32, attend_case, check_attend, check_matvec, gen, half_step, make_codes
 
 pytestmark = pytest.mark.gpu
 
@@ -55,6 +55,39 @@ def test_fp32_products_keep_their_bits(n, k, vectors, group, zeros):
   x = torch.randn(vectors, k, generator=g, device=DEV)
   got = W4Matrix.from_codes(packed, scales, zeros=z, in_features=k, group=group).matvec(x)
   assert rms_error(got, product_64(codes, scales, z, group, x)) <= fp32_rms_bound(group, scales.shape[1], zeros)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_the_largest_finite_vectors(dtype, group):
+  """Vectors up to the largest finite number: the result is finite wherever the formula's is, whatever a group's sums before scaling are."""
+  from tacotron_amd.w4 import W4Matrix
+  most = torch.finfo(dtype).max
+  for vectors, n, k in ((1, 40, 300), (17, 4200, 256), (2, 8300, 129)):
+    for zeros in (False, True):
+      g = gen(n + group)
+      codes, packed, scales, z = make_codes(n, k, group, F32, zeros, g)
+      scales *= 2.0 ** -20            # sums of |w x| stay below the largest number
+      W = W4Matrix.from_codes(packed, scales, zeros=z, in_features=k, group=group)
+      x = (1 - torch.rand(vectors, k, generator=g, device=DEV) / 4).to(dtype) * most
+      for signed in (x, x * torch.where(torch.rand(x.shape, generator=g, device=DEV) < 0.5, -1, 1).to(dtype)):
+        got = W.matvec(signed)
+        assert torch.isfinite(got).all(), (vectors, n, zeros)
+        check_matvec(codes, scales, z, group, None, signed, got)
+
+
+@pytest.mark.parametrize("size", [1e-29, 1e-32])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_small_vectors_keep_their_bits(dtype, size):
+  """Small vectors are as exact as any: the last bits of an fp32 number of 1e-32, 1e-39, times a code held as 2^-12 are subnormal numbers."""
+  from tacotron_amd.w4 import W4Matrix
+  g = gen(2)
+  for zeros in (False, True):
+    codes, packed, scales, z = make_codes(200, 512, 64, F32, zeros, g)
+    W = W4Matrix.from_codes(packed, scales, zeros=z, in_features=512, group=64)
+    x = (torch.randn(4, 512, generator=g, device=DEV) * size).to(dtype)
+    error = rms_error(W.matvec(x), product_64(codes, scales, z, 64, x))
+    assert error <= fp32_rms_bound(64, 8, zeros) + (half_step(BF16) if dtype == BF16 else 0), (zeros, error)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
