@@ -336,8 +336,9 @@ int taco_kv_attend(const taco_kv_cache* cache, const taco_kv_attend_args* args, 
  * They depend on the sizes only, not on the lengths. */
 int64_t taco_kv_attend_workspace(const taco_kv_cache* cache, const taco_kv_attend_args* args);
 
-/* Waits for the work enqueued on `stream`, reads and clears the cache's flags: TACO_ERANGE when a call has met a table
- * entry that is no page, or a position or length outside the table. */
+/* Waits for the work enqueued on `stream`, reads the cache's flags and clears those it reports: TACO_ERANGE when a call has met a
+ * table entry that is no page, or a position or length outside the table.  What calls on other streams, which it does not wait for,
+ * set afterwards is left for the next check. */
 int taco_kv_status(const taco_kv_cache* cache, void* stream);
 
 /* A matrix [n_rows, n_cols] of 4-bit codes: W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), zero = 8

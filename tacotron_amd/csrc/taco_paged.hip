@@ -925,17 +925,24 @@ extern "C" int taco_kv_attend(const taco_kv_cache* c, const taco_kv_attend_args*
   return by_types(c, t->dtype, p.group, [&](auto ty, auto ca, auto dp, auto qt) { return launch_attend<ty.value, ca.value, dp.value, qt.value>(a, p, (hipStream_t)stream); });
 }
 
+namespace {
+
+// Clears what has been reported and nothing else: a call on another stream may have set a bit since the flags were read.
+__global__ void taco_kv_clear_flags_kernel(uint32_t* flags, uint32_t reported) { atomicAnd(flags, ~reported); }
+
+}  // namespace
+
 extern "C" int taco_kv_status(const taco_kv_cache* c, void* stream) {
   if (!c || !c->flags) TACO_FAIL(TACO_EINVAL, "taco_kv_status: NULL argument");
   DeviceScope on_device(c->device);
   TACO_HIP(on_device.status);
   hipStream_t s = (hipStream_t)stream;
   uint32_t flags = 0;
-  const uint32_t zero = 0;
   TACO_HIP(hipMemcpyAsync(&flags, c->flags, 4, hipMemcpyDeviceToHost, s));
   TACO_HIP(hipStreamSynchronize(s));
   if (!flags) return TACO_OK;
-  TACO_HIP(hipMemcpyAsync(c->flags, &zero, 4, hipMemcpyHostToDevice, s));
+  taco_kv_clear_flags_kernel<<<dim3(1), dim3(1), 0, s>>>(c->flags, flags);
+  TACO_HIP(hipGetLastError());
   TACO_HIP(hipStreamSynchronize(s));
   TACO_FAIL(TACO_ERANGE, "%s%s%s", flags & TACO_KV_BAD_PAGE ? "a table entry is no page of the cache" : "",
             flags == (TACO_KV_BAD_PAGE | TACO_KV_BAD_PLACE) ? "; " : "", flags & TACO_KV_BAD_PLACE ? "a position or length lies outside the table" : "");

@@ -305,5 +305,6 @@ class PagedCache:
 
   def check(self) -> None:
     """Waits for the current stream and raises an IndexError if a call since the last check has met a table entry that is
-    no page of the cache, or a position or length outside its table (such tokens are neither stored nor seen)."""
+    no page of the cache, or a position or length outside its table (such tokens are neither stored nor seen).  What calls on
+    other streams find after that is raised by the next check."""
     _lib.check(self._lib.taco_kv_status(self._ref, _lib.raw_stream(self._c.device)))

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from matvec_bounds import fp32_rms_bound, rms_error
-from test_gpu_step_ops import BF16, DEV, E4M3, F16, F32, attend_case, check_attend, check_matvec, gen, half_step, make_codes
+from test_gpu_step_ops import (BF16, DEV, E4M3, F16, F32, attend_case, check_attend, check_matvec, gen,
+                               half_step, make_cache, make_codes)
 
 pytestmark = pytest.mark.gpu
 
@@ -139,3 +140,27 @@ def test_every_form_of_the_attention(dtype, held, heads, hq, d, page, lens, wind
   cache.check()
   check_attend(cache, q, table, lens, d ** -0.5, window, got)
   assert cache.attend(q, table, lens_dev, window=window, out=q) is q and torch.equal(q, got[0])
+
+
+def test_a_report_from_another_stream_is_not_lost():
+  """What a call on another stream sets while a check reads and clears is reported by this check or the next."""
+  cache = make_cache(4, 16, 2, 64, BF16, gen(1))
+  k = torch.zeros(1, 2, 64, dtype=BF16, device=DEV)
+  ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+  no_page, some_page, first, far = ints(-1)[None], ints(0)[None], ints(0), ints(1000)
+  side = torch.cuda.Stream(device=DEV)
+  torch.cuda.synchronize()
+  for i in range(400):
+    with torch.cuda.stream(side):
+      torch.cuda._sleep(1 + 500 * i)
+      cache.append(k, k, some_page, far)            # outside the table
+    cache.append(k, k, no_page, first)              # no page
+    said = ""
+    for _ in range(2):
+      try:
+        cache.check()
+      except IndexError as e:
+        said += str(e)
+      torch.cuda.synchronize()
+    assert "page" in said and "outside" in said, (i, said)
+    cache.check()
