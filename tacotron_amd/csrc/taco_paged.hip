@@ -854,10 +854,10 @@ int plan_attend(const taco_kv_cache* c, const taco_kv_attend_args* t, Plan& p) {
   if (rc != TACO_OK) return rc;
   const int64_t rows = (int64_t)t->n_seqs * c->n_heads * p.q_tiles;
   const int64_t tiles = ((int64_t)t->table_width * c->page_size + p.tt - 1) / p.tt;       // of a row, at most
-  // no more workgroups than there are parts when every row is cut on its own; if all of those are there and a table has room for
-  // one part of a row only, every row is finished by its workgroup and the second kernel is left out
+  // no more workgroups than there are parts when every row is cut on its own; shares are whole parts, so where a table has room for
+  // one part of a row only, every row is finished by one workgroup and the second kernel is left out
   const int64_t parts = ((tiles < 1 ? 1 : tiles) + PART - 1) / PART, most = rows * parts;
-  p.join = parts > 1 || most > p.workgroups;
+  p.join = parts > 1;
   if (most < p.workgroups) p.workgroups = (uint32_t)most;
   p.bytes = (rows + 1) / 2 * 16 + (int64_t)2 * p.workgroups * p.held * (2 + p.dp) * 4;
   return TACO_OK;

@@ -1,5 +1,6 @@
 """The self-attention step's operators on the GPU, continued: every form of the kernels, the ends of the range of numbers, calls
 that meet each other.  Tolerances as in test_gpu_step_ops.py."""
+import ctypes as C
 
 import pytest
 import torch
@@ -140,6 +141,30 @@ def test_every_form_of_the_attention(dtype, held, heads, hq, d, page, lens, wind
   cache.check()
   check_attend(cache, q, table, lens, d ** -0.5, window, got)
   assert cache.attend(q, table, lens_dev, window=window, out=q) is q and torch.equal(q, got[0])
+
+
+def captured_nodes(call):
+  """How many nodes a call leaves in a graph."""
+  graph = torch.cuda.CUDAGraph(keep_graph=True)
+  with torch.cuda.graph(graph):
+    keep = call()  # noqa: F841
+  n = C.c_size_t()
+  hip = C.CDLL("libamdhip64.so")
+  assert hip.hipGraphGetNodes(C.c_void_p(graph.raw_cuda_graph()), None, C.byref(n)) == 0
+  return n.value
+
+
+def test_one_kernel_where_every_row_is_one_part():
+  """A table with room for one part of a row (128 tokens, 64 in fp32) leaves nothing to join, however many rows there are."""
+  for dtype, held, page, width, kernels in ((BF16, BF16, 64, 2, 1), (F32, F32, 16, 4, 1), (BF16, BF16, 64, 3, 2), (F32, F32, 16, 5, 2)):
+    cache = make_cache(4, page, 8, 64, held, gen(1))
+    table = torch.tensor([[0, 1, 2, 3, 0]], dtype=torch.int32, device=DEV)[:, :width].expand(600, width)
+    lens = torch.full((600,), width * page - 5, dtype=torch.int32, device=DEV)
+    q = torch.randn(600, 8, 64, generator=gen(2), device=DEV).to(dtype)
+    got = cache.attend(q, table, lens, return_lse=True)
+    for at in (slice(0, 3), slice(597, 600)):
+      check_attend(cache, q[at], table[at], [width * page - 5] * 3, 0.125, 0, (got[0][at], got[1][at]))
+    assert captured_nodes(lambda: cache.attend(q, table, lens)) == kernels, (dtype, width)
 
 
 def test_a_report_from_another_stream_is_not_lost():
