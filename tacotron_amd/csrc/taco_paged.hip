@@ -459,11 +459,11 @@ struct Utterances {
     if (b < a.n_seqs) {
       len = a.lens[b];
       const int64_t room = (int64_t)a.table_width * a.page16.div * 16;
+      low = a.window > 0 && len > a.window ? len - a.window : 0;      // the window ends at the length given, wherever the table does
       if (len < 0 || len > room) {
         if (flag) atomicOr(a.flags, TACO_KV_BAD_PLACE);
         len = len < 0 ? 0 : (int)room;
       }
-      low = a.window > 0 ? max(0, len - a.window) : 0;
       tiles = len > low ? (uint32_t)((len + TT - 1) / TT - low / TT) : 1;
     }
     parts = (tiles + PART - 1) / PART;

@@ -1,6 +1,7 @@
 """The self-attention step's operators on the GPU, continued: every form of the kernels, the ends of the range of numbers, calls
 that meet each other.  Tolerances as in test_gpu_step_ops.py."""
 import ctypes as C
+import math
 
 import pytest
 import torch
@@ -165,6 +166,22 @@ def test_one_kernel_where_every_row_is_one_part():
     for at in (slice(0, 3), slice(597, 600)):
       check_attend(cache, q[at], table[at], [width * page - 5] * 3, 0.125, 0, (got[0][at], got[1][at]))
     assert captured_nodes(lambda: cache.attend(q, table, lens)) == kernels, (dtype, width)
+
+
+def test_window_of_a_length_beyond_the_table():
+  """The window ends at the length that was given; of what it shows, the table's tokens are seen."""
+  cache, q, table, _ = attend_case(BF16, BF16, 2, 4, 64, 16, [48, 48, 48, 48], 0)
+  short = table[:, :3]
+  ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=DEV)  # noqa: E731
+  o, lse = cache.attend(q, short, ints(100, 108, 40, 2 ** 31 - 1), window=60, return_lse=True)
+  with pytest.raises(IndexError):
+    cache.check()
+  want, want_lse = cache.attend(q, short, ints(48, 0, 40, 0), window=8, return_lse=True)
+  whole, whole_lse = cache.attend(q, short, ints(48, 48, 40, 0), return_lse=True)
+  cache.check()
+  assert torch.equal(o[:2], want[:2]) and torch.equal(lse[:2], want_lse[:2])       # tokens 40 .. 47, none
+  assert torch.equal(o[2:], whole[2:]) and torch.equal(lse[2:], whole_lse[2:])
+  assert not o[3].any() and bool((lse[3] == -math.inf).all())
 
 
 def test_a_report_from_another_stream_is_not_lost():
