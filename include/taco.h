@@ -364,7 +364,8 @@ int taco_qmat_pack(const taco_qmat* m, const uint8_t* codes, int64_t code_stride
 
 /* Codes, scales (and zero points with has_zeros) of a matrix of weights [n_rows, weight_stride] of type `dtype`, as
  * taco_qmat_pack takes them: the scale is max|w| / 7 of its group, or (max - min) / 15 with zero points (the interval holds
- * 0), rounded to scale_dtype; a code is the nearest one to its weight.  Weights must be finite. */
+ * 0), rounded to scale_dtype (to its largest finite number if it is larger); a code is the nearest one to its weight.  Weights must be
+ * finite. */
 int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_stride, int32_t dtype, uint8_t* codes,
                        int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
 

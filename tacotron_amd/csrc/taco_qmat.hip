@@ -110,7 +110,8 @@ __global__ __launch_bounds__(64) void taco_qmat_quantize_kernel(const QuantizePa
   }
   // without zero points the codes 1 .. 15 stand for -7 .. 7 scales; with them 0 .. 15 span lo .. hi
   float scale = a.zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
-  if (a.scale_dtype == TACO_F16) scale = (float)(_Float16)scale;
+  if (scale == __builtin_inff()) scale = hi / 15.0f - lo / 15.0f;      // the range of finite weights may be infinite, a fifteenth is not
+  if (a.scale_dtype == TACO_F16) scale = (float)(_Float16)fminf(scale, 65504.0f);      // codes at the ends stand for what is beyond
   else if (a.scale_dtype == TACO_BF16) scale = (float)(__bf16)scale;
   const float zero = a.zeros ? (scale > 0.0f ? fminf(fmaxf(rintf(-lo / scale), 0.0f), 15.0f) : 0.0f) : 8.0f;
   uint32_t byte = 0;

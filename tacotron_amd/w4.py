@@ -39,7 +39,7 @@ def quantize(weight: torch.Tensor, group: int = 128, symmetric: bool = True,
              scale_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor, Optional[torch.Tensor]]:
   """Codes, scales and zero points (None if ``symmetric``) of ``weight`` [out, in], which must be finite, as
   ``W4Matrix.from_codes`` takes them: the scale of a group is max|w| / 7, or (max - min) / 15 with zero points, and a code the
-  nearest to its weight.  ``scale_dtype`` defaults to the weight's type."""
+  nearest to its weight.  ``scale_dtype`` defaults to the weight's type; a scale beyond its range becomes its largest number."""
   device = _on_gpu(weight, "weight")
   if weight.dim() != 2 or weight.dtype not in _FLOATS or weight.numel() == 0:
     raise ValueError(f"weight must be a float matrix, got {weight.dtype} {tuple(weight.shape)}")

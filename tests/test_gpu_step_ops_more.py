@@ -107,6 +107,28 @@ def test_as_many_vectors_as_there_may_be(dtype):
   assert bool(torch.isfinite(got).all())
 
 
+def test_quantize_weights_whose_scale_leaves_its_type():
+  """Finite weights give finite matrices: a range beyond fp32, scales beyond float16."""
+  from tacotron_amd import w4
+  most = torch.finfo(F32).max
+  w = torch.tensor([[most, -most, most / 2, 0.0], [most, -most / 3, 1.0, -1.0], [3.0, -4.0, 0.5, 0.0]], device=DEV)
+  codes, scales, zeros = w4.quantize(w, 32, symmetric=False)
+  s = torch.stack([(w.double().amax(1) - w.double().amin(1)) / 15], 1)
+  assert ((scales.double() - s).abs() <= 3 * 2.0 ** -24 * s).all()
+  unpacked = torch.stack([codes & 15, codes >> 4], -1).flatten(1).double()
+  back = (unpacked - zeros.double()) * scales.double()
+  assert ((back - w.double()).abs() <= s * (0.5 + 0.5 + 1e-5)).all()          # the zero point is rounded, and the code
+  w = torch.tensor([[1e6, -2e6, 3e5, 0.0], [4e5, 1.0, -4e5, 65504.0]], device=DEV)
+  for symmetric in (True, False):
+    codes, scales, zeros = w4.quantize(w, 32, symmetric=symmetric, scale_dtype=F16)
+    assert scales[0, 0].item() == 65504 and bool(torch.isfinite(scales).all())
+    z = torch.full((2, 1), 8.0) if symmetric else zeros.cpu().float()
+    want = ((w.cpu() / scales.cpu().float()).round() + z).clamp(0, 15)
+    assert torch.equal(torch.stack([codes & 15, codes >> 4], -1).flatten(1).cpu().float(), want)
+    W = w4.W4Matrix.from_codes(codes, scales, zeros=zeros, in_features=4, group=32)
+    assert bool(torch.isfinite(W.matvec(torch.ones(1, 4, device=DEV))).all())
+
+
 # ---- attend -------------------------------------------------------------------------------------------------------------
 
 EDGES = [0, 1, 15, 16, 17, 33, 64, 65, 128, 129, 300]
