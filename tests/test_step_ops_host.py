@@ -1,7 +1,11 @@
 """The self-attention step's operators without a GPU, continued: what a build depends on, and the bounds that the GPU tests use."""
+import os
+import subprocess
+
 import pytest
 import torch
 
+from conftest import ROOT
 from matvec_bounds import fp32_rms_bound, rms_error
 
 
@@ -37,3 +41,10 @@ def test_the_bound_of_fp32_products_tells_lost_bits(group, zeros, n, k, vectors)
   assert torch.equal(cut(x, 3), x)
   for wrong in (cut(x, 2).double() @ w.t(), x.half().double() @ w.t(), want.half()):
     assert rms_error(wrong, want) > 2 * bound
+
+
+def test_objects_are_built_again_when_the_flags_change():
+  """The flags stand in the makefiles (in the product's, the one that keeps packed fp32 arithmetic out)."""
+  for folder, target in (("tacotron_amd/csrc", "taco_qmat.o"), ("tests/support", "libhold_cu.so"), ("tests/support", "libplace.so")):
+    told = subprocess.check_output(["make", "-n", "-W", "Makefile", "-C", os.path.join(ROOT, folder), target], text=True)
+    assert "-o " + target in told, (folder, told)
