@@ -48,3 +48,11 @@ def test_objects_are_built_again_when_the_flags_change():
   for folder, target in (("tacotron_amd/csrc", "taco_qmat.o"), ("tests/support", "libhold_cu.so"), ("tests/support", "libplace.so")):
     told = subprocess.check_output(["make", "-n", "-W", "Makefile", "-C", os.path.join(ROOT, folder), target], text=True)
     assert "-o " + target in told, (folder, told)
+
+
+def test_a_build_compiles_whatever_is_there(monkeypatch):
+  import __graft_entry__
+  calls = []
+  monkeypatch.setattr(__graft_entry__.subprocess, "check_call", lambda args, **kw: calls.append(args))
+  __graft_entry__.build()
+  assert len(calls) == 3 and all(args[0] == "make" and "-B" in args for args in calls)
