@@ -1,5 +1,6 @@
 import json
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -14,6 +15,13 @@ GOLDEN = os.path.join(ROOT, "tests", "golden")
 
 def pytest_configure(config):
   config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
+
+
+@pytest.fixture(scope="session", autouse=True)
+def host_library(request):
+  """The address arithmetic that CPU tests load is compiled from the kernels' header as it is now (a GPU run loads what was built)."""
+  if any(item.get_closest_marker("gpu") is None for item in request.session.items):
+    subprocess.check_call(["make", "-C", os.path.join(ROOT, "tests", "support"), "libplace.so"], stdout=subprocess.DEVNULL)
 
 
 def load_golden(name):

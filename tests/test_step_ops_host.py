@@ -56,3 +56,9 @@ def test_a_build_compiles_whatever_is_there(monkeypatch):
   monkeypatch.setattr(__graft_entry__.subprocess, "check_call", lambda args, **kw: calls.append(args))
   __graft_entry__.build()
   assert len(calls) == 3 and all(args[0] == "make" and "-B" in args for args in calls)
+
+
+def test_the_host_library_is_as_new_as_its_sources():
+  """What test_step_ops.py loads has been compiled from the kernels' header as it is now."""
+  age = lambda *path: os.path.getmtime(os.path.join(ROOT, *path))  # noqa: E731
+  assert age("tests", "support", "libplace.so") >= max(age("tests", "support", "place.cpp"), age("tacotron_amd", "csrc", "taco_place.h"))
