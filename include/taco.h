@@ -285,7 +285,7 @@ typedef struct taco_kv_append_args {
   const void* k;              /* [n_tokens, n_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
   const void* v;
   const void* q;              /* [n_tokens, n_q_heads, head_dim] or NULL */
-  void* q_out;                /* like q (may be q itself), its rows apart from each other and from k and v; NULL when q is */
+  void* q_out;                /* like q (may be q itself, else apart from it), its rows apart from each other and from k and v; NULL when q is */
   const int32_t* table;       /* [n_seqs, table_width] */
   const int32_t* past;        /* [n_seqs] tokens of each utterance that the cache holds already */
   const int32_t* offsets;     /* [n_seqs + 1], rising: rows offsets[b] .. offsets[b+1]-1 are utterance b's new tokens;
@@ -304,13 +304,13 @@ typedef struct taco_kv_append_args {
  * (x c - y s, y c + x s), in fp32, rounded once to the cache's type - for TACO_E4M3 after the division by the head's
  * scale, what is beyond +-448 becoming +-448.  Rows in front of offsets[0] or behind offsets[n_seqs] are left alone in
  * q_out.  A token whose page is not in the table, or whose table entry is no page, is not written and sets a flag.  No two
- * tokens of a call may have the same place (what is stored there is undefined then), and k, v and q may not lie in the pages
- * that are written.  At most 2^24 - 1 tokens at once. */
+ * tokens of a call may have the same place (what is stored there is undefined then), the cache's k and v may not share memory, and k, v and q may not lie in the
+ * pages that are written.  At most 2^24 - 1 tokens at once. */
 int taco_kv_append(const taco_kv_cache* cache, const taco_kv_append_args* args, void* stream);
 
 typedef struct taco_kv_attend_args {
   const void* q;              /* [n_seqs, n_q_heads, head_dim], unit stride in head_dim, 16-byte aligned rows */
-  void* out;                  /* like q (may be q itself), its rows apart from each other */
+  void* out;                  /* like q (may be q itself, else apart from it), its rows apart from each other */
   float* lse;                 /* [n_seqs, n_q_heads] or NULL */
   const int32_t* table;       /* [n_seqs, table_width] */
   const int32_t* lens;        /* [n_seqs] tokens of each utterance, the new one included */

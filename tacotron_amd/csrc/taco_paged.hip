@@ -56,6 +56,7 @@ __device__ __forceinline__ void store_cache(char* p, float (&x)[8], float scale)
 // every thread takes pieces of 16 elements of a head: both halves of 8 pairs, or 16 elements that are only copied.
 // Bound by moving the rows: 6200 tokens of ragged prompts, 32 + 2 x 8 heads of 128 from bfloat16 into an 8-bit cache, 144 MB, take
 // 29.8 us = 4.8 TB/s, what a large copy reaches; one token of 64 utterances 4.1 us, mostly the launch and one round trip to memory.
+// Beyond 256 pieces a token takes turns, a round trip each: 128 + 2 x 8 heads of 128 5.9 us, 384 + 2 x 16 heads of 256 (26 turns) 20.7.
 template <int T, int C>
 __global__ __launch_bounds__(256) void taco_kv_append_kernel(const AppendParams a) {
   __shared__ float cs[128], sn[128];
@@ -191,7 +192,11 @@ struct State {
 // K and V serve 16 * QT query heads of a cache head; further ones read them again.  With more than 16, QT = 2 pays where reading
 // is the bound (16 x 16384 tokens, 2 heads of 128 in bfloat16, 64 query heads: 82 us with QT = 1, 71 with 2; 16 x 60000 tokens
 // of 64 elements, 64 query heads over one: 144 and 90), not for fp32, whose products are slower than its reading (48 query
-// heads over 2 of 128: 78 and 86).
+// heads over 2 of 128: 78 and 86).  Heads of more than 128 elements take all 512 registers with QT = 2 and spill 19 of them in 16-bit caches,
+// one workgroup to a CU; it still pays (16 x 16384 tokens, 2 heads of 256 in bfloat16, 34 / 128 query heads: 165 / 301 us with QT = 1, 125 / 186
+// with 2; heads of 144 124 / 222 and 88 / 152; of 256 in 8 bits 103 / 183 and 74 / 137).
+// Heads run in the next larger instance of 64, 128, 256 elements, whose products meet zeros behind the head: 16 x 16384 tokens, 8 query heads over
+// 2 in bfloat16, heads of 64 / 80 / 96 / 128 / 192 / 256: 4.5 / 4.9 / 5.3 / 5.7 / 4.7 / 5.2 TB/s.
 template <int T, int C, int DP, int QT>
 struct Attend {
   static constexpr int CB = taco_size_of<C>;

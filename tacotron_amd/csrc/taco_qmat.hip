@@ -93,7 +93,8 @@ struct QuantizeParams {
 };
 
 // One wave per group of a row, two columns per lane: the group's extremes by six exchanges, then every lane rounds its own.  Done
-// once per matrix and kept simple.
+// once per matrix and kept simple: a wave has 64 to 512 bytes to read, and starting so many is the bound (28672 x 8192 from fp32 or bfloat16: 0.5 ms in
+// groups of 128, 1.8 in groups of 32).
 __global__ __launch_bounds__(64) void taco_qmat_quantize_kernel(const QuantizeParams a) {
   const int64_t row = blockIdx.x;
   const int group = blockIdx.y, lane = threadIdx.x;

@@ -344,6 +344,11 @@ int launch(const taco_qmat_multiply_params& a, hipStream_t s) {
 // one; not in groups of 32, 4096 x 4097 19.5 and 22.1).  fp32 vectors need three times the registers and take a tile at a time (28672 x
 // 4096 with 32: 50 us, two tiles and two row blocks 80), two only where four row blocks have no room (groups of 32, 28672 x 4096
 // with 17: 73 and 81).
+// Some of these have too few registers by a handful.  Two tiles with four row blocks (fp32 scales in groups of 64 5 to 13 short, other
+// scales of vectors at odd addresses up to 12) win all the same: 28672 x 4096 with 32 bfloat16 vectors in groups of 64 with fp32 scales 32 us, with
+// two row blocks 48, at odd addresses with zero points 42 and 60.  Sixteen waves with two row blocks in groups of 64 with fp32 scales (5 to 9 short)
+// do not: eight would take 13.8 us instead of 17.7 for 4160 x 4096 with sixteen fp32 vectors, 9.3 instead of 10.5 with bfloat16 ones, 16.9 and
+// 17.1 for 8192 x 8192 with one; with 16-bit scales one vector takes 8.9 and 8.7, 15.9 and 16.0.
 template <int T, int GPB, int S>
 int launch(const taco_qmat_multiply_params& a, int n_cu, hipStream_t s) {
   constexpr bool FOUR = !(GPB == 4 && S == TACO_F32);

@@ -64,7 +64,8 @@ class PagedCache:
   ``table[b, t // page_size]``.  ``dtype`` is float32, float16, bfloat16 or float8_e4m3fn; the last holds x / scale with
   one scale per head (``k_scale`` / ``v_scale``, float32 [n_heads], 1 when not given).
 
-  Pages and tables are the caller's to hand out; calls on different streams may overlap as long as none writes a page that
+  ``append`` takes any number of new tokens of an utterance, ``attend`` the queries of one, its last: the attention among a
+  prompt's own tokens is not offered here.  Pages and tables are the caller's to hand out; calls on different streams may overlap as long as none writes a page that
   another reads or writes.  Inference only: results carry no gradients."""
 
   def __init__(self, n_pages: int, page_size: int, n_heads: int, head_dim: int, dtype: torch.dtype = torch.float32,
@@ -183,8 +184,8 @@ class PagedCache:
     multiple of 16 up to head_dim) rotates the first R elements of every key head by ``position * inv_freq``: the pairs
     (i, i + R/2), or (2i, 2i + 1) with ``interleaved``.  ``q`` [tokens, query heads, head_dim] are queries of the same
     tokens, rotated likewise: returned, or written to ``out`` (which may be ``q``).  Rows that belong to no utterance are
-    left as they were in ``out``.  No two tokens of a call may go to the same place, and ``out`` may overlap no other
-    input."""
+    left as they were in ``out``.  No two tokens of a call may go to the same place, keys and values of the cache may not share
+    memory, and ``out`` may be ``q`` but else overlap no input."""
     interleaved = bool(interleaved)
     key = (_form(k), _form(v), _form(table), _form(past), None if q is None else _form(q), None if offsets is None else _form(offsets),
            None if inv_freq is None else _form(inv_freq), interleaved, None if out is None else _form(out))
@@ -248,7 +249,7 @@ class PagedCache:
              return_lse: bool = False, out: Optional[torch.Tensor] = None):
     """Attention of one new token per utterance: ``q`` [utterances, query heads, head_dim] over the first ``lens`` (int32
     [utterances]) tokens of each, or the last ``window`` of those; ``scale`` defaults to head_dim ** -0.5.  Query head h
-    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q``) and, with
+    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q`` and else overlaps no input) and, with
     ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
     (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
     infinite value that is seen gives NaN."""
