@@ -1,5 +1,6 @@
 """What the repository holds."""
 import os
+import shutil
 import subprocess
 
 import pytest
@@ -8,10 +9,10 @@ from conftest import ROOT
 
 
 def test_no_compiled_code_is_under_version_control():
-  if not os.path.isdir(os.path.join(ROOT, ".git")):
+  if not os.path.exists(os.path.join(ROOT, ".git")) or not shutil.which("git"):
     pytest.skip("not a checkout")
   built = []
-  for name in subprocess.check_output(["git", "-C", ROOT, "ls-files", "-z"], text=True).split("\0"):
+  for name in subprocess.check_output(["git", "-c", "safe.directory=*", "-C", ROOT, "ls-files", "-z"], text=True).split("\0"):
     path = os.path.join(ROOT, name)
     if name and os.path.isfile(path):
       with open(path, "rb") as f:
