@@ -304,8 +304,8 @@ typedef struct taco_kv_append_args {
  * (x c - y s, y c + x s), in fp32, rounded once to the cache's type - for TACO_E4M3 after the division by the head's
  * scale, what is beyond +-448 becoming +-448.  Rows in front of offsets[0] or behind offsets[n_seqs] are left alone in
  * q_out.  A token whose page is not in the table, or whose table entry is no page, is not written and sets a flag.  No two
- * tokens of a call may have the same place (what is stored there is undefined then), the cache's k and v may not share memory, and k, v and q may not lie in the
- * pages that are written.  At most 2^24 - 1 tokens at once. */
+ * tokens of a call may have the same place (what is stored there is undefined then), the cache's k and v may not share memory, and
+ * k, v and q may not lie in the pages that are written.  At most 2^24 - 1 tokens at once. */
 int taco_kv_append(const taco_kv_cache* cache, const taco_kv_append_args* args, void* stream);
 
 typedef struct taco_kv_attend_args {
@@ -370,7 +370,8 @@ int taco_qmat_quantize(const taco_qmat* m, const void* weights, int64_t weight_s
                        int64_t code_stride, void* scales, int64_t scale_stride, uint8_t* zeros, int64_t zero_stride, void* stream);
 
 /* y[v] = W x[v] + bias for n_vectors vectors x [n_vectors, x_stride] of type `dtype` (TACO_F32, TACO_F16, TACO_BF16), y
- * [n_vectors, y_stride] of the same type; sums are fp32, rounded once (an infinite element gives NaN).  At most 2^20 vectors.  y may not overlap x.  W is read again
+ * [n_vectors, y_stride] of the same type; sums are fp32, rounded once (an infinite element gives NaN; of float32 and bfloat16 results
+ * below 5e-35 the last bits are lost).  At most 2^20 vectors.  y may not overlap x.  W is read again
  * for every 32 vectors (for every 16 of a matrix with few rows or of fp32 vectors). */
 int taco_qmat_multiply(const taco_qmat* m, const void* x, int64_t x_stride, void* y, int64_t y_stride, int32_t n_vectors,
                        int32_t dtype, void* stream);

@@ -81,7 +81,8 @@ struct Operand<TACO_F32, ODD> {
 // such products: 2^-15 of the result measured.)
 // A group's sums are formed before its scale makes them small: up to 31 * 128 times the largest element for bfloat16, 15 * 128 for
 // fp32.  So that they stay below the largest fp32 number whatever the vectors, bfloat16 and fp32 codes are held 2^-12 times as large and
-// the finished sum is multiplied by 2^12 (float16 vectors end at 65504).  Both are exact, down to products of 2^-149.
+// the finished sum is multiplied by 2^12 (float16 vectors end at 65504).  Both are exact as long as sums are normal numbers: results
+// below 2^-114 = 5e-35 are held to 2^-138 instead of 2^-149.
 // Bound by reading the codes: 28672 x 8192 for one bfloat16 vector, 122 MB, takes 26.4 us = 4.6 TB/s (a large copy reaches 4.7; the
 // same loads without any product 23.7 us); groups of 32 columns 35 us, where scaling the sums binds; an fp32 vector 45 us
 // (groups of 64), where splitting it and converting the codes does (a byte at a time 54).  4096 x 4096 4.4 us, 4096 x 1558 for sixteen fp32 vectors 6.1 us, 80 x 1558 for one

@@ -65,8 +65,8 @@ class PagedCache:
   one scale per head (``k_scale`` / ``v_scale``, float32 [n_heads], 1 when not given).
 
   ``append`` takes any number of new tokens of an utterance, ``attend`` the queries of one, its last: the attention among a
-  prompt's own tokens is not offered here.  Pages and tables are the caller's to hand out; calls on different streams may overlap as long as none writes a page that
-  another reads or writes.  Inference only: results carry no gradients."""
+  prompt's own tokens is not offered here.  Pages and tables are the caller's to hand out; calls on different streams may
+  overlap as long as none writes a page that another reads or writes.  Inference only: results carry no gradients."""
 
   def __init__(self, n_pages: int, page_size: int, n_heads: int, head_dim: int, dtype: torch.dtype = torch.float32,
                device: Union[torch.device, str, int] = "cuda", k_scale: Optional[torch.Tensor] = None,
@@ -249,8 +249,8 @@ class PagedCache:
              return_lse: bool = False, out: Optional[torch.Tensor] = None):
     """Attention of one new token per utterance: ``q`` [utterances, query heads, head_dim] over the first ``lens`` (int32
     [utterances]) tokens of each, or the last ``window`` of those; ``scale`` defaults to head_dim ** -0.5.  Query head h
-    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q`` and else overlaps no input) and, with
-    ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
+    reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q``
+    and else overlaps no input) and, with ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
     (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
     infinite value that is seen gives NaN."""
     scale, window = None if scale is None else float(scale), int(window)      # numbers: a tensor would stand for itself in the key
