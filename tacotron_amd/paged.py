@@ -250,9 +250,9 @@ class PagedCache:
     """Attention of one new token per utterance: ``q`` [utterances, query heads, head_dim] over the first ``lens`` (int32
     [utterances]) tokens of each, or the last ``window`` of those; ``scale`` defaults to head_dim ** -0.5.  Query head h
     reads cache head ``h // (query heads / n_heads)``.  Returns the output like ``q`` (or in ``out``, which may be ``q``
-    and else overlaps no input) and, with ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query heads].  An utterance that sees nothing
-    (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at and behind ``lens`` does not matter; an
-    infinite value that is seen gives NaN."""
+    and else overlaps no input) and, with ``return_lse``, the logarithm of the softmax's sum, float32 [utterances, query
+    heads].  An utterance that sees nothing (length 0, or no score above -inf) gets zeros and -inf.  What lies in slots at
+    and behind ``lens`` does not matter; an infinite value that is seen gives NaN."""
     scale, window = None if scale is None else float(scale), int(window)      # numbers: a tensor would stand for itself in the key
     key = (_form(q), _form(table), _form(lens), scale, window, None if out is None else _form(out))
     found = self._attend_forms.get(key)
